@@ -149,6 +149,12 @@ EXT_SIGNATURES = {
     "cngpt_cuda_loader_reset": (I, [VP]),
     "cngpt_cuda_loader_num_batches": (C.c_size_t, [VP]),
     "cngpt_cuda_loader_free": (None, [VP]),
+    "cngpt_cuda_sample": (I, [VP, L, I, I, VP, VP, VP, VP, VP, VP, VP]),
+    "cngpt_cuda_topk": (I, [VP, L, I, I, I, VP, VP]),
+    "cngpt_cuda_distill": (I, [VP, L, I, I, VP, VP, I, VP, F, F, F, VP, VP, VP, L]),
+    "cngpt_cuda_prefix_attention_workspace": (C.c_size_t, [I, I, I, I, I, I]),
+    "cngpt_cuda_prefix_attention": (I, [VP, L, VP, VP, L, I, VP, VP, L, L, VP, I, VP, L, I, I, I, I, F, VP,
+                                        C.c_size_t]),
 }
 
 

@@ -119,4 +119,35 @@ int attention_decode_at(const float *q, long ldq, const float *kcache, const flo
                         const int *pos_dev, float *out, int B, int C, int H, float *part,
                         cudaStream_t s);
 
+// ------------------------------------------------- the model's distribution
+// Rows of logits [rows, V] with pitch ldl. Definitions and edge cases: the
+// comments of the matching entry points in cngpt_cuda.h. Arguments are checked
+// by the callers.
+constexpr int SAMPLE_MAX_VOCAB = 262144;
+constexpr int TOPK_MAX = 1024;
+// next (may be null): max(token, 0), a row index that is safe to embed
+int sample_rows(const float *logits, long ldl, int rows, int V, const float *temperature, const int *top_k,
+                const float *top_p, const float *min_p, const float *u, int *tokens, float *logprob, int *next,
+                cudaStream_t s);
+int topk_rows(const float *logits, long ldl, int rows, int V, int k, float *values, int *indices, cudaStream_t s);
+int distill_rows(const float *logits, long ldl, int rows, int V, const float *tv, const int *ti, int k,
+                 const int *targets, float tau, float alpha, float scale, float *row_loss, float *dlogits, long ldd,
+                 cudaStream_t s);
+// loss = scale * sum of row_loss, in a fixed order
+int distill_loss_sum(const float *row_loss, int rows, float scale, float *loss, cudaStream_t s);
+
+// Decode attention of B sequences over a shared prefix and their own suffixes
+// (cngpt_cuda_prefix_attention).
+struct PrefixAttn {
+    const float *q, *pk, *pv, *sk, *sv;
+    long ldq, ldp, lds, seq_stride, ldo;
+    int P, S;              // prefix length, suffix capacity
+    const int *suffix_len;  // device, [B]
+    float *out;
+    int B, H, Hk, hs;
+    float scale;
+};
+size_t prefix_attention_ws_bytes(int B, int H, int Hk, int hs, int P, int S);
+int prefix_attention(const PrefixAttn &a, void *ws, cudaStream_t s);
+
 }  // namespace cg

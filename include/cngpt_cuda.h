@@ -103,6 +103,97 @@ int cngpt_cuda_layernorm_bwd_noalloc(const float *dout, const float *x, const fl
                                      const float *mean, const float *rstd,
                                      float *dx, float *dw, float *db, int T, int C);
 
+/* ---- sampling from given random numbers -------------------------------------
+ * The reference samples on the host, one row at a time, from rand()
+ * (src/model.c:927-989: temperature and top-k). This draws one token for each
+ * of `rows` rows of logits [rows, vocab] (row pitch ld >= vocab) on the device,
+ * from one given uniform number u[r] in [0, 1) per row. All pointers are device
+ * pointers; every parameter array has one entry per row and may be NULL, which
+ * switches its filter off (temperature: 1).
+ *
+ * The weight of token i is w_i = exp((l_i - max l) / temperature). Tokens are
+ * ranked by logit, equal logits by index (the lower first), and filtered in
+ * this order:
+ *   top_k > 0          the first top_k of the ranking stay;
+ *   top_p < 1          of what top_k left, a token stays while the weights ranked
+ *                      before it sum to less than top_p times the sum of all that
+ *                      top_k left (the first always stays);
+ *   min_p > 0          of what is left, a token stays if w_i >= min_p (min_p above
+ *                      1 counts as 1).
+ * The token is the first one, in index order, whose cumulative weight over the
+ * kept tokens exceeds u times their sum. temperature <= 0 (or NaN) takes the
+ * first of the ranking. Logits that are -inf or NaN are never drawn; +inf
+ * logits share the draw equally. A row in which nothing can be drawn gives
+ * token -1 and logprob -inf. Weights and sums are held in 64 bits, so the token
+ * does not depend on rounding unless u lies within about 1e-9 of a border, and
+ * the same inputs always give the same token.
+ * logprob (may be NULL): the log of the probability with which the token was
+ * drawn among the kept ones (0 for a greedy row).
+ * 1 <= vocab <= 262144. */
+int cngpt_cuda_sample(const float *logits, long ld, int rows, int vocab, const float *temperature,
+                      const int *top_k, const float *top_p, const float *min_p, const float *u,
+                      int *tokens, float *logprob);
+
+/* ---- the k largest logits of every row --------------------------------------
+ * values [rows, k] falling, indices [rows, k]; equal values are ordered by index
+ * (the lower first), NaN ranks below -inf, and -0 equals (and is returned as) 0.
+ * 1 <= k <= min(vocab, 1024). Device pointers. */
+int cngpt_cuda_topk(const float *logits, long ld, int rows, int vocab, int k, float *values, int *indices);
+
+/* ---- distillation from a teacher's top logits ----------------------------------
+ * The reference trains on hard targets alone (cross_entropy_fwd / _bwd,
+ * src/ops.c:499-590). Here a row of student logits x also learns from a list of
+ * k teacher logits top_val [rows, k] at tokens top_idx [rows, k]:
+ *   p = softmax(top_val / temperature) over the row's list,
+ *   q_t = softmax(x / t) over the vocabulary,
+ *   row_loss = alpha temperature^2 sum p (log p - log q_temperature)
+ *            + (1 - alpha) (-log q_1[target]),
+ *   loss = scale * sum of row_loss,
+ *   dlogits = scale (alpha temperature (q_temperature - p)
+ *                    + (1 - alpha) (q_1 - onehot(target))).
+ * List entries whose token lies outside [0, vocab) or whose value is -inf or
+ * NaN count for nothing; a token that is listed twice has the sum of both
+ * probabilities. A row without a list entry has no soft part, a row whose
+ * target lies outside [0, vocab) no hard part, a row with neither has loss 0
+ * and gradient 0, and so has a row whose logits are all -inf. A vocabulary entry
+ * of -inf has probability 0 (a teacher's token or a target there makes the loss
+ * +inf, its gradient stays finite); NaN logits give NaN.
+ * targets may be NULL when alpha == 1, top_val and top_idx when alpha == 0 or
+ * k == 0. dlogits NULL computes the loss alone; dlogits may be logits itself
+ * (with ldd == ld), else the two must not overlap. Columns from vocab to ldd
+ * are left as they are. loss: one float, row_loss: rows floats, both written.
+ * temperature > 0, 0 <= alpha <= 1, 0 <= k <= 1024. All pointers are device
+ * pointers. The result does not depend on the order in which blocks run. */
+int cngpt_cuda_distill(const float *logits, long ld, int rows, int vocab, const float *top_val,
+                       const int *top_idx, int k, const int *targets, float temperature, float alpha,
+                       float scale, float *loss, float *row_loss, float *dlogits, long ldd);
+
+/* ---- decode attention of sequences that share a prefix -------------------------
+ * One query per sequence: q [B, n_head, hs] (row pitch ldq), over the keys of a
+ * prefix that all B sequences share, pk / pv [prefix_len, n_kv_head, hs] (row
+ * pitch ldp), and of each sequence's own suffix, sk / sv
+ * [B][max_suffix, n_kv_head, hs] (row pitch lds, seq_stride floats from one
+ * sequence to the next), of which sequence b has the first suffix_len[b]
+ * (device array; clamped to [0, max_suffix]):
+ *   out[b, h] = softmax over both of (scale q . k) times v,
+ * query head h reading key/value head h / (n_head / n_kv_head). The prefix is
+ * read once for all sequences. A sequence that sees no key gets zeros. What is
+ * read has to be finite and below 1e37 in size; keys behind a sequence's suffix
+ * and the gaps that the pitches leave are not read.
+ * out [B, n_head, hs] (row pitch ldo). hs <= 256; 0 <= prefix_len, max_suffix;
+ * pk / pv may be NULL when prefix_len == 0, sk / sv when max_suffix == 0 (and
+ * suffix_len then too). All pointers are device pointers.
+ * ws: device workspace of at least prefix_attention_workspace bytes, 16-byte
+ * aligned, its contents unspecified before and after; calls that may overlap
+ * on the GPU (other streams, two captured graphs) need one each. Computed at
+ * fp32 level in the 3xTF32 and FP32 modes and in one TF32 pass in TF32 mode. */
+size_t cngpt_cuda_prefix_attention_workspace(int B, int n_head, int n_kv_head, int hs, int prefix_len,
+                                             int max_suffix);
+int cngpt_cuda_prefix_attention(const float *q, long ldq, const float *pk, const float *pv, long ldp,
+                                int prefix_len, const float *sk, const float *sv, long lds, long seq_stride,
+                                const int *suffix_len, int max_suffix, float *out, long ldo, int B, int n_head,
+                                int n_kv_head, int hs, float scale, void *ws, size_t ws_bytes);
+
 /* ---- training ------------------------------------------------------------
  * One full step of the reference's train loop (src/cngpt.c:154-163):
  * zero_grad, forward, backward, [DP allreduce], AdamW with clipping.
