@@ -152,6 +152,9 @@ EXT_SIGNATURES = {
     "cngpt_cuda_sample": (I, [VP, L, I, I, VP, VP, VP, VP, VP, VP, VP]),
     "cngpt_cuda_topk": (I, [VP, L, I, I, I, VP, VP]),
     "cngpt_cuda_distill": (I, [VP, L, I, I, VP, VP, I, VP, F, F, F, VP, VP, VP, L]),
+    "cngpt_cuda_distill_step": (I, [C.POINTER(GPT), VP, VP, VP, VP, I, F, F, I, I, F, F, F, F, F, F, VP]),
+    "cngpt_cuda_generate_shared": (I, [C.POINTER(GPT), C.POINTER(FastCtx), VP, I, I, I, F, I, F, F, VP, VP]),
+    "cngpt_cuda_teacher_topk": (I, [C.POINTER(GPT), C.POINTER(FastCtx), VP, I, I, I, VP, VP]),
     "cngpt_cuda_prefix_attention_workspace": (C.c_size_t, [I, I, I, I, I, I]),
     "cngpt_cuda_prefix_attention": (I, [VP, L, VP, VP, L, I, VP, VP, L, L, VP, I, VP, L, I, I, I, I, F, VP,
                                         C.c_size_t]),

@@ -49,4 +49,8 @@ struct Stage {
 
 void *op_scratch(size_t bytes);
 
+// ERR_ARG (with fn and name in the message) unless p is a 4-byte aligned
+// pointer to memory that kernels on the current device reach (ops_ext_abi.cu)
+int dev_ptr(const char *fn, const char *name, const void *p);
+
 }  // namespace cg

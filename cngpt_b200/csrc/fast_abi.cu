@@ -37,8 +37,22 @@ void drop_graph(FastDev *d) {
     d->graph_params = nullptr;
 }
 
+void drop_shared(FastDev *d) {
+    if (d->sh_graph) cudaGraphExecDestroy(d->sh_graph);
+    d->sh_graph = nullptr;
+    d->sh_graph_params = nullptr;
+}
+
 int fast_resize(FastCtx *f, FastDev *d, const GPT *m, int B, int T, bool managed) {
-    if (f->x && f->B == B && f->T == T) return OK;
+    const int dims[4] = {m->cfg.n_embd, m->cfg.vocab_size, m->cfg.n_layer, m->cfg.n_head};
+    const bool same_model = !memcmp(dims, d->dims, sizeof(dims));
+    if (f->x && f->B == B && f->T == T && same_model) return OK;
+    if (!same_model) {  // a model of another shape: the caches are laid out anew too
+        drop_shared(d);
+        d->kv_B = d->kv_T = 0;
+        d->sh_n = d->sh_S = 0;
+        memcpy(d->dims, dims, sizeof(dims));
+    }
     cudaStreamSynchronize(g_stream);
     if (d->cap_stream) cudaStreamSynchronize(d->cap_stream);
     drop_graph(d);  // the captured step holds the scratch addresses
@@ -297,6 +311,13 @@ extern "C" void fast_free(FastCtx *f) {
         dev_free(d->mk_bar);
         dev_free(d->mk_trace);
         drop_graph(d);
+        drop_shared(d);
+        dev_free(d->sh_f);
+        dev_free(d->sh_i);
+        dev_free(d->sh_u);
+        dev_free(d->sh_gen);
+        dev_free(d->sh_ws);
+        dev_free(d->tk_logits);
         if (d->ev_a) cudaEventDestroy(d->ev_a);
         if (d->ev_b) cudaEventDestroy(d->ev_b);
         if (d->cap_stream) cudaStreamDestroy(d->cap_stream);
@@ -437,6 +458,290 @@ extern "C" int cngpt_cuda_generate(GPT *m, FastCtx *f, const int *prompt, int B,
     for (int b = 0; b < B; ++b)
         for (int i = 0; i < n_new; ++i) out_tokens[(size_t)b * n_new + i] = h[(size_t)i * B + b];
     if (d->mk_trace && n_new > 1) report_trace(d->mk_trace, m->cfg.n_layer);
+    return OK;
+}
+
+// -------------------------------------------- sampling from one prompt
+// cngpt_cuda_generate_shared: n sequences continue one prompt. The prompt is
+// prefilled once and its cache is shared; every step runs one row per sequence
+// through the stack, attends to the prompt's keys and to the sequence's own
+// suffix, and draws the tokens on the device, so the steps replay as one graph.
+namespace cg {
+namespace {
+
+struct Shared {  // the pieces of FastDev::sh_f and sh_i
+    float *x, *ln, *qkv, *att, *hid, *logits, *stats, *temp, *top_p, *min_p, *kc, *vc;
+    int *ctr, *next, *top_k, *slen, *ticket;
+    long ldlog;
+    size_t floats, ints;
+};
+
+// ctr: [0] position of the incoming token, [1] step, [2] its place in the suffix
+Shared shared_layout(const GPT *m, int n, int S, float *f, int *i) {
+    Shared b{};
+    size_t at = 0, ia = 0;
+    auto take = [&](size_t k) { float *p = f + at; at += (k + 63) / 64 * 64; return p; };
+    auto itake = [&](size_t k) { int *p = i + ia; ia += (k + 63) / 64 * 64; return p; };
+    const size_t C = m->cfg.n_embd, N = n;
+    b.ldlog = ((long)m->cfg.vocab_size + 3) / 4 * 4;
+    b.x = take(N * C);
+    b.ln = take(N * C);
+    b.qkv = take(N * 3 * C);
+    b.att = take(N * C);
+    b.hid = take(N * 4 * C);
+    b.logits = take(N * b.ldlog);
+    b.stats = take(32);
+    b.temp = take(N);
+    b.top_p = take(N);
+    b.min_p = take(N);
+    b.kc = take((size_t)m->cfg.n_layer * N * S * C);
+    b.vc = take((size_t)m->cfg.n_layer * N * S * C);
+    b.ctr = itake(4);
+    b.next = itake(N);
+    b.top_k = itake(N);
+    b.slen = itake(N);
+    b.ticket = itake(4);
+    b.floats = at;
+    b.ints = ia;
+    return b;
+}
+
+int shared_prepare(const GPT *m, FastDev *d, int n, int S, int T, int n_new, cudaStream_t s, Shared *out) {
+    if (d->sh_n != n || d->sh_S < S || !d->sh_f) {
+        CG_CUDA(cudaStreamSynchronize(s));
+        drop_shared(d);
+        dev_free(d->sh_f);
+        dev_free(d->sh_i);
+        d->sh_f = nullptr;
+        d->sh_i = nullptr;
+        d->sh_n = d->sh_S = 0;
+        const Shared sz = shared_layout(m, n, S, nullptr, nullptr);
+        CG_TRY(dev_alloc((void **)&d->sh_f, sz.floats * sizeof(float), false));
+        CG_TRY(dev_alloc((void **)&d->sh_i, sz.ints * sizeof(int), false));
+        d->sh_n = n;
+        d->sh_S = S;
+    }
+    const size_t need = (size_t)n_new * n;
+    if (need > d->sh_gen_cap) {
+        CG_CUDA(cudaStreamSynchronize(s));
+        drop_shared(d);
+        dev_free(d->sh_u);
+        dev_free(d->sh_gen);
+        d->sh_u = nullptr;
+        d->sh_gen = nullptr;
+        d->sh_gen_cap = 0;
+        CG_TRY(dev_alloc((void **)&d->sh_u, need * sizeof(float), false));
+        CG_TRY(dev_alloc((void **)&d->sh_gen, need * sizeof(int), false));
+        d->sh_gen_cap = need;
+    }
+    const int C = m->cfg.n_embd, H = m->cfg.n_head;
+    const size_t ws = prefix_attention_ws_bytes(n, H, H, C / H, T, d->sh_S);
+    if (ws > d->sh_ws_bytes || !d->sh_ws) {
+        CG_CUDA(cudaStreamSynchronize(s));
+        drop_shared(d);
+        dev_free(d->sh_ws);
+        d->sh_ws = nullptr;
+        d->sh_ws_bytes = 0;
+        CG_TRY(dev_alloc(&d->sh_ws, ws, false));
+        d->sh_ws_bytes = ws;
+    }
+    *out = shared_layout(m, n, d->sh_S, d->sh_f, d->sh_i);
+    return OK;
+}
+
+SampleRows shared_sample(const GPT *m, const FastDev *d, const Shared &b, const float *logits, long ldl) {
+    SampleRows a{logits, ldl, d->sh_n, m->cfg.vocab_size, b.temp, b.top_k, b.top_p, b.min_p, d->sh_u, d->sh_gen, nullptr};
+    a.next = b.next;
+    a.step = b.ctr + 1;
+    return a;
+}
+
+// One token for each sequence: the incoming tokens b.next sit at position
+// ctr[0] and place ctr[2] of their suffixes, slen = ctr[2] + 1.
+int shared_step(const GPT *m, FastDev *d, const Shared &b, int T, cudaStream_t s) {
+    const int C = m->cfg.n_embd, V = m->cfg.vocab_size, L = m->cfg.n_layer, H = m->cfg.n_head, n = d->sh_n;
+    const GPTWeights *w = &m->params;
+    CG_TRY(embed_fwd_at(b.next, w->wte, w->wpe, b.x, n, C, b.ctr, s));
+    const size_t pre = (size_t)d->kv_B * d->kv_T * C, per = (size_t)n * d->sh_S * C;
+    const bool st = n <= 8;  // LayerNorm statistics handed between the GEMVs, as in decode_step
+    float *st_attn = b.stats, *st_mlp = b.stats + 16;
+    auto resid = [&](const float *bias, float *stats, int *ticket) {
+        GemmEpi e = epi_resid_inplace(b.x, C, bias);
+        if (st) {
+            e.ln_stats_out = stats;
+            e.ln_ticket = ticket;
+        }
+        return e;
+    };
+    for (int l = 0; l < L; l++) {
+        GemmEpi eq = epi_store(b.qkv, 3 * C, w->c_attn_b[l]);
+        eq.kc = b.kc + l * per;
+        eq.vc = b.vc + l * per;
+        eq.kv_ld = (long)d->sh_S * C;
+        eq.kv_pos = b.ctr + 2;
+        eq.kv_C = C;
+        CG_TRY(gemm_ln(b.x, C, w->ln1_w[l], w->ln1_b[l], (st && l > 0) ? st_mlp : nullptr, b.ln, w->c_attn_w[l], C, n,
+                       3 * C, C, eq, s));
+        PrefixAttn a{b.qkv, d->kc + l * pre, d->vc + l * pre, eq.kc, eq.vc, 3L * C, C, C, eq.kv_ld, C, T, d->sh_S, b.slen,
+                     b.att, n, H, H, C / H, 1.0f / sqrtf((float)(C / H))};
+        CG_TRY(prefix_attention(a, d->sh_ws, s));
+        CG_TRY(gemm(b.att, C, false, w->c_proj_w[l], C, false, n, C, C, resid(w->c_proj_b[l], st_attn, b.ticket), s));
+        CG_TRY(gemm_ln(b.x, C, w->ln2_w[l], w->ln2_b[l], st ? st_attn : nullptr, b.ln, w->mlp_fc_w[l], C, n, 4 * C, C,
+                       epi_gelu_only(b.hid, 4 * C, w->mlp_fc_b[l]), s));
+        CG_TRY(gemm(b.hid, 4 * C, false, w->mlp_proj_w[l], 4 * C, false, n, C, 4 * C,
+                    resid(w->mlp_proj_b[l], st_mlp, b.ticket + 1), s));
+    }
+    CG_TRY(gemm_ln(b.x, C, w->ln_f_w, w->ln_f_b, (st && L > 0) ? st_mlp : nullptr, b.ln, w->wte, C, n, V, C,
+                   epi_store(b.logits, b.ldlog, nullptr), s));
+    CG_TRY(sample_rows(shared_sample(m, d, b, b.logits, b.ldlog), s));
+    return shared_advance(b.ctr, b.slen, n, s);
+}
+
+int capture_shared(const GPT *m, FastDev *d, const Shared &b, int T) {
+    if (d->sh_graph && d->sh_graph_params == m->param_buf && d->sh_graph_kc == d->kc && d->sh_graph_T == T &&
+        d->sh_graph_kvT == d->kv_T && d->sh_graph_prec == precision())
+        return OK;
+    drop_shared(d);
+    cudaGraph_t g = nullptr;
+    CG_CUDA(cudaStreamBeginCapture(d->cap_stream, cudaStreamCaptureModeThreadLocal));
+    const int st = shared_step(m, d, b, T, d->cap_stream);
+    const cudaError_t e = cudaStreamEndCapture(d->cap_stream, &g);
+    if (st != OK || e != cudaSuccess) {
+        if (g) cudaGraphDestroy(g);
+        cudaGetLastError();
+        if (st == OK) set_last_error(ERR_CUDA, "shared decode graph capture: %s", cudaGetErrorString(e));
+        return st != OK ? st : ERR_CUDA;
+    }
+    const cudaError_t ei = cudaGraphInstantiate(&d->sh_graph, g, 0);
+    cudaGraphDestroy(g);
+    if (ei != cudaSuccess) {
+        d->sh_graph = nullptr;
+        set_last_error(ERR_CUDA, "shared decode graph instantiate: %s", cudaGetErrorString(ei));
+        return ERR_CUDA;
+    }
+    d->sh_graph_params = m->param_buf;
+    d->sh_graph_kc = d->kc;
+    d->sh_graph_T = T;
+    d->sh_graph_kvT = d->kv_T;
+    d->sh_graph_prec = precision();
+    return OK;
+}
+
+}  // namespace
+}  // namespace cg
+
+extern "C" int cngpt_cuda_generate_shared(GPT *m, FastCtx *f, const int *prompt, int T, int n_seq, int n_new,
+                                          float temperature, int top_k, float top_p, float min_p, const float *u,
+                                          int *out_tokens) {
+    ModelCtx *c = model_ctx(m);
+    if (!c) return ERR_STATE;
+    const int V = m->cfg.vocab_size, hs = m->cfg.n_head > 0 ? m->cfg.n_embd / m->cfg.n_head : 0;
+    if (T <= 0 || n_seq <= 0 || n_new <= 0 || (long)T + n_new - 1 > m->cfg.block_size || n_seq > 4096) {
+        set_last_error(ERR_ARG, "generate_shared: T=%d n_seq=%d (at most 4096) n_new=%d exceeds block_size %d", T, n_seq,
+                       n_new, m->cfg.block_size);
+        return ERR_ARG;
+    }
+    if (!f || !prompt || !u || !out_tokens || V > SAMPLE_MAX_VOCAB || hs < 1 || hs > 256) {
+        set_last_error(ERR_ARG, "generate_shared: NULL argument, or vocab %d > %d, or head size %d > 256", V,
+                       SAMPLE_MAX_VOCAB, hs);
+        return ERR_ARG;
+    }
+    cudaStream_t s = g_stream;
+    FastDev *d = fast_dev(f, true);
+    CG_TRY(kv_prepare(m, f, d, 1, T, 1, c->managed, s));
+    Shared b;
+    CG_TRY(shared_prepare(m, d, n_seq, std::max(1, n_new - 1), T, n_new, s, &b));
+    const int *tok = nullptr;
+    CG_TRY(stage_tokens(prompt, (size_t)T, &d->tok, &d->tok_cap, &tok, s));
+    // the step parameters of every sequence and the counters before the first draw
+    const size_t n = n_seq;
+    std::vector<float> fl(n, temperature), tp(n, top_p), mp(n, min_p);
+    std::vector<int> tk(n, top_k), one(n, 0);
+    const int ctr0[3] = {T - 1, 0, -1};
+    CG_CUDA(cudaMemcpyAsync(b.temp, fl.data(), n * 4, cudaMemcpyHostToDevice, s));
+    CG_CUDA(cudaMemcpyAsync(b.top_p, tp.data(), n * 4, cudaMemcpyHostToDevice, s));
+    CG_CUDA(cudaMemcpyAsync(b.min_p, mp.data(), n * 4, cudaMemcpyHostToDevice, s));
+    CG_CUDA(cudaMemcpyAsync(b.top_k, tk.data(), n * 4, cudaMemcpyHostToDevice, s));
+    CG_CUDA(cudaMemcpyAsync(b.slen, one.data(), n * 4, cudaMemcpyHostToDevice, s));
+    CG_CUDA(cudaMemcpyAsync(b.ctr, ctr0, sizeof(ctr0), cudaMemcpyHostToDevice, s));
+    CG_CUDA(cudaMemsetAsync(b.ticket, 0, 4 * sizeof(int), s));
+    CG_CUDA(cudaMemcpyAsync(d->sh_u, u, n * n_new * 4, cudaMemcpyDefault, s));
+    CG_TRY(fast_forward(m, f, d, tok, 1, T, true, s));
+    CG_TRY(sample_rows(shared_sample(m, d, b, f->logits, 0), s));  // every sequence draws from the prompt's logits
+    CG_TRY(shared_advance(b.ctr, b.slen, n_seq, s));
+    if (n_new > 1) {
+        CG_CUDA(cudaEventRecord(d->ev_a, s));
+        CG_CUDA(cudaStreamWaitEvent(d->cap_stream, d->ev_a, 0));
+        CG_TRY(shared_step(m, d, b, T, d->cap_stream));  // eager first step (warms the kernels)
+        if (n_new > 2) {
+            CG_TRY(capture_shared(m, d, b, T));
+            for (int i = 2; i < n_new; ++i) CG_CUDA(cudaGraphLaunch(d->sh_graph, d->cap_stream));
+        }
+        CG_CUDA(cudaEventRecord(d->ev_b, d->cap_stream));
+        CG_CUDA(cudaStreamWaitEvent(s, d->ev_b, 0));
+    }
+    std::vector<int> h(n * n_new);
+    CG_CUDA(cudaMemcpyAsync(h.data(), d->sh_gen, h.size() * 4, cudaMemcpyDeviceToHost, s));
+    CG_CUDA(cudaStreamSynchronize(s));
+    CG_TRY(check_device_error());
+    for (size_t q = 0; q < n; ++q)
+        for (int i = 0; i < n_new; ++i) out_tokens[q * n_new + i] = h[(size_t)i * n + q];
+    return OK;
+}
+
+// ------------------------------------------------- a teacher's top logits
+// The inference forward for every position (fast_forward without the last
+// layer's restriction to final rows), then the LM head and the row ranking one
+// stretch of rows at a time: the [B*T, V] logits never exist as a whole.
+namespace cg {
+namespace {
+constexpr int TK_ROWS = 1024;
+}
+}  // namespace cg
+
+extern "C" int cngpt_cuda_teacher_topk(GPT *m, FastCtx *f, const int *tokens, int B, int T, int k, float *values,
+                                       int *indices) {
+    ModelCtx *c = model_ctx(m);
+    if (!c) return ERR_STATE;
+    const int C = m->cfg.n_embd, V = m->cfg.vocab_size, L = m->cfg.n_layer, H = m->cfg.n_head;
+    if (!f || !tokens || B <= 0 || T <= 0 || T > m->cfg.block_size || k < 1 || k > V || k > TOPK_MAX) {
+        set_last_error(ERR_ARG, "teacher_topk: bad shape B=%d T=%d (block %d) k=%d (at most min(vocab=%d, %d))", B, T,
+                       m->cfg.block_size, k, V, TOPK_MAX);
+        return ERR_ARG;
+    }
+    CG_TRY(dev_ptr("teacher_topk", "values", values));
+    CG_TRY(dev_ptr("teacher_topk", "indices", indices));
+    cudaStream_t s = g_stream;
+    FastDev *d = fast_dev(f, true);
+    CG_TRY(fast_resize(f, d, m, B, T, c->managed));
+    const long BT = (long)B * T, ldl = ((long)V + 3) / 4 * 4;
+    const size_t need = (size_t)std::min<long>(BT, TK_ROWS) * ldl;
+    if (need > d->tk_cap) {
+        CG_CUDA(cudaStreamSynchronize(s));
+        dev_free(d->tk_logits);
+        d->tk_logits = nullptr;
+        d->tk_cap = 0;
+        CG_TRY(dev_alloc((void **)&d->tk_logits, need * sizeof(float), false));
+        d->tk_cap = need;
+    }
+    const int *tok = nullptr;
+    CG_TRY(stage_tokens(tokens, (size_t)BT, &d->tok, &d->tok_cap, &tok, s));
+    const GPTWeights *w = &m->params;
+    CG_TRY(embed_fwd(tok, w->wte, w->wpe, f->x, (int)BT, T, C, 0, s));
+    for (int l = 0; l < L; l++) {
+        CG_TRY(layernorm_fwd(f->x, C, w->ln1_w[l], w->ln1_b[l], f->ln, C, f->mean, f->rstd, (int)BT, C, s));
+        CG_TRY(gemm(f->ln, C, false, w->c_attn_w[l], C, false, (int)BT, 3 * C, C, epi_store(f->qkv, 3 * C, w->c_attn_b[l]),
+                    s));
+        CG_TRY(attention_fwd(f->qkv, f->aout, nullptr, B, T, C, H, s));
+        CG_TRY(block_tail(m, l, f, f->x, f->aout, (int)BT, s));
+    }
+    CG_TRY(layernorm_fwd(f->x, C, w->ln_f_w, w->ln_f_b, f->ln, C, f->mean, f->rstd, (int)BT, C, s));
+    for (long r = 0; r < BT; r += TK_ROWS) {
+        const int rows = (int)std::min<long>(TK_ROWS, BT - r);
+        CG_TRY(gemm(f->ln + r * C, C, false, w->wte, C, false, rows, V, C, epi_store(d->tk_logits, ldl, nullptr), s));
+        CG_TRY(topk_rows(d->tk_logits, ldl, rows, V, k, values + r * k, indices + r * k, s));
+    }
+    if (c->managed) CG_CUDA(cudaStreamSynchronize(s));
     return OK;
 }
 

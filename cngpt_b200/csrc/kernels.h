@@ -125,16 +125,29 @@ int attention_decode_at(const float *q, long ldq, const float *kcache, const flo
 // by the callers.
 constexpr int SAMPLE_MAX_VOCAB = 262144;
 constexpr int TOPK_MAX = 1024;
-// next (may be null): max(token, 0), a row index that is safe to embed
-int sample_rows(const float *logits, long ldl, int rows, int V, const float *temperature, const int *top_k,
-                const float *top_p, const float *min_p, const float *u, int *tokens, float *logprob, int *next,
-                cudaStream_t s);
+struct SampleRows {
+    const float *logits;
+    long ldl;  // 0: every row draws from the same logits
+    int rows, V;
+    const float *temperature;
+    const int *top_k;
+    const float *top_p, *min_p, *u;
+    int *tokens;
+    float *logprob;
+    int *next = nullptr;        // max(token, 0): a row that is safe to embed
+    const int *step = nullptr;  // u and tokens are indexed [*step * rows + row]
+};
+int sample_rows(const SampleRows &a, cudaStream_t s);
 int topk_rows(const float *logits, long ldl, int rows, int V, int k, float *values, int *indices, cudaStream_t s);
 int distill_rows(const float *logits, long ldl, int rows, int V, const float *tv, const int *ti, int k,
                  const int *targets, float tau, float alpha, float scale, float *row_loss, float *dlogits, long ldd,
                  cudaStream_t s);
 // loss = scale * sum of row_loss, in a fixed order
 int distill_loss_sum(const float *row_loss, int rows, float scale, float *loss, cudaStream_t s);
+
+// counters of the shared-prefix decode loop: ctr[0..2] (position, step, suffix
+// position) and every suffix length advance by one
+int shared_advance(int *ctr, int *suffix_len, int n, cudaStream_t s);
 
 // Decode attention of B sequences over a shared prefix and their own suffixes
 // (cngpt_cuda_prefix_attention).

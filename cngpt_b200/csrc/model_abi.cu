@@ -300,8 +300,18 @@ int resize_acts(GPT *m, ModelCtx *c, int B, int T) {
 // one pass then turns the rows into dlogits in place. The arena's logits and
 // probs slots are not written. Otherwise logits and probs land in the arena
 // as in the reference.
+// distill (training step against a teacher's lists): the logits go into the
+// dlogits buffer too, and one pass over their rows leaves the gradient of the
+// distillation loss there.
+struct Distill {
+    const float *top_val;
+    const int *top_idx;
+    int k;
+    float temperature, alpha;
+};
+
 int forward(GPT *m, ModelCtx *c, const int *tokens, const int *targets, int B, int T, bool want_grad,
-            cudaStream_t s, bool fused_ce = false) {
+            cudaStream_t s, bool fused_ce = false, const Distill *distill = nullptr) {
     const int C = m->cfg.n_embd, V = m->cfg.vocab_size, L = m->cfg.n_layer, H = m->cfg.n_head;
     const int BT = B * T;
     if (B <= 0 || T <= 0 || T > m->cfg.block_size || H <= 0 || C % H != 0) {
@@ -314,7 +324,7 @@ int forward(GPT *m, ModelCtx *c, const int *tokens, const int *targets, int B, i
     size_t cap = c->extra_BT;
     CG_TRY(stage_tokens(tokens, BT, &c->tok, &cap, &tok, s));
     CG_TRY(stage_tokens(targets, BT, &c->tgt, &cap, &tgt, s));
-    const bool training = targets && m->cfg.dropout > 0.0f;
+    const bool training = (targets || distill) && m->cfg.dropout > 0.0f;
     GPTActivations *a = &m->acts;
     GPTWeights *w = &m->params;
     CG_TRY(embed_fwd(tok, w->wte, w->wpe, a->emb, BT, T, C, 0, s));
@@ -369,6 +379,21 @@ int forward(GPT *m, ModelCtx *c, const int *tokens, const int *targets, int B, i
     c->dlogits_valid = false;
     c->fwd_targets = targets;
     float *rowterm = c->scratch;
+    if (distill) {
+        GemmEpi e;
+        e.mode = EPI_STORE;
+        e.D = c->dlogits;
+        e.ldd = c->ldlog;
+        CG_TRY(gemm(a->ln_f_out, C, false, w->wte, C, false, BT, V, C, e, s));
+        const float scale = 1.0f / (float)BT;
+        CG_TRY(distill_rows(c->dlogits, c->ldlog, BT, V, distill->top_val, distill->top_idx, distill->k, tgt,
+                            distill->temperature, distill->alpha, scale, rowterm, c->dlogits, c->ldlog, s));
+        if (c->ldlog > V)
+            CG_CUDA(cudaMemset2DAsync(c->dlogits + V, c->ldlog * sizeof(float), 0, (c->ldlog - V) * sizeof(float), BT, s));
+        CG_TRY(distill_loss_sum(rowterm, BT, scale, &c->dev_scalars[0], s));
+        c->dlogits_valid = true;
+        return OK;
+    }
     if (fused_ce && targets && want_grad) {
         // src/model.c:612-623 and 644-665 in two kernels: logits with row
         // statistics, then loss terms and dlogits
@@ -917,19 +942,14 @@ extern "C" void gpt_adamw(GPT *m, float lr, float beta1, float beta2, float eps,
 
 // ============================================================ cngpt_cuda.h (model)
 
-extern "C" int cngpt_cuda_train_step(GPT *m, const int *tokens, const int *targets, int B, int T,
-                                     float lr, float beta1, float beta2, float eps, float wd,
-                                     float grad_clip, float *loss_out) {
-    ModelCtx *c = model_ctx(m);
-    if (!c) return ERR_STATE;
-    if (!targets) {
-        set_last_error(ERR_ARG, "train_step: targets required");
-        return ERR_ARG;
-    }
+namespace cg {
+namespace {
+int train_step(GPT *m, ModelCtx *c, const int *tokens, const int *targets, const Distill *distill, int B, int T, float lr,
+               float beta1, float beta2, float eps, float wd, float grad_clip, float *loss_out) {
     cudaStream_t s = g_stream;
     const bool dp = c->world > 1 && c->nccl_comm;
     CG_CUDA(cudaMemsetAsync(m->grad_buf, 0, (size_t)m->n_params * sizeof(float), s));
-    CG_TRY(forward(m, c, tokens, targets, B, T, true, s, true));
+    CG_TRY(forward(m, c, tokens, targets, B, T, true, s, true, distill));
     if (dp) {
         // the reported loss is the mean over the global batch (every rank has B*T rows)
         CG_CUDA(cudaEventRecord(c->ev_ready, s));
@@ -944,6 +964,41 @@ extern "C" int cngpt_cuda_train_step(GPT *m, const int *tokens, const int *targe
         *loss_out = *c->host_loss;
     }
     return OK;
+}
+}  // namespace
+}  // namespace cg
+
+extern "C" int cngpt_cuda_train_step(GPT *m, const int *tokens, const int *targets, int B, int T,
+                                     float lr, float beta1, float beta2, float eps, float wd,
+                                     float grad_clip, float *loss_out) {
+    ModelCtx *c = model_ctx(m);
+    if (!c) return ERR_STATE;
+    if (!targets) {
+        set_last_error(ERR_ARG, "train_step: targets required");
+        return ERR_ARG;
+    }
+    return train_step(m, c, tokens, targets, nullptr, B, T, lr, beta1, beta2, eps, wd, grad_clip, loss_out);
+}
+
+extern "C" int cngpt_cuda_distill_step(GPT *m, const int *tokens, const int *targets, const float *top_val,
+                                       const int *top_idx, int k, float temperature, float alpha, int B, int T, float lr,
+                                       float beta1, float beta2, float eps, float wd, float grad_clip, float *loss_out) {
+    ModelCtx *c = model_ctx(m);
+    if (!c) return ERR_STATE;
+    if (!tokens || (alpha < 1.0f && !targets) || k < 0 || k > TOPK_MAX || !(temperature > 0.0f) || !std::isfinite(temperature) ||
+        !(alpha >= 0.0f && alpha <= 1.0f)) {
+        set_last_error(ERR_ARG, "distill_step: tokens and (with alpha=%g < 1) targets required, k=%d in [0, %d], "
+                       "temperature=%g positive", (double)alpha, k, TOPK_MAX, (double)temperature);
+        return ERR_ARG;
+    }
+    const bool soft = k > 0 && alpha > 0.0f;
+    if (soft) {
+        CG_TRY(dev_ptr("distill_step", "top_val", top_val));
+        CG_TRY(dev_ptr("distill_step", "top_idx", top_idx));
+    }
+    const Distill ds{top_val, top_idx, soft ? k : 0, temperature, alpha};
+    return train_step(m, c, tokens, alpha < 1.0f ? targets : nullptr, &ds, B, T, lr, beta1, beta2, eps, wd, grad_clip,
+                      loss_out);
 }
 
 extern "C" int cngpt_cuda_last_loss(GPT *m, float *loss_out) {

@@ -43,6 +43,7 @@ struct ModelCtx {
 };
 
 struct FastDev {
+    int dims[4] = {0, 0, 0, 0};  // n_embd, vocab, layers, heads that the buffers are sized for
     size_t cap_BT = 0;
     int cap_B = 0;
     float *xl = nullptr, *al = nullptr;  // last-row gathers [B, C]
@@ -68,6 +69,24 @@ struct FastDev {
     const void *graph_params = nullptr;
     int graph_B = 0, graph_T = 0, graph_prec = -1;
     const float *graph_logits = nullptr;
+    // cngpt_cuda_generate_shared: n sequences over the prompt's cache (kc / vc
+    // of batch 1) with their own suffixes [L][n][S][C]; one allocation each
+    // for the floats and the ints, carved up by shared_prepare
+    int sh_n = 0, sh_S = 0;
+    float *sh_f = nullptr;
+    int *sh_i = nullptr;
+    float *sh_u = nullptr;  // [n_new][n] uniform numbers
+    int *sh_gen = nullptr;  // [n_new][n] tokens
+    size_t sh_gen_cap = 0;
+    void *sh_ws = nullptr;  // attention workspace
+    size_t sh_ws_bytes = 0;
+    cudaGraphExec_t sh_graph = nullptr;
+    const void *sh_graph_params = nullptr;
+    const float *sh_graph_kc = nullptr;
+    int sh_graph_T = 0, sh_graph_kvT = 0, sh_graph_prec = -1;
+    // cngpt_cuda_teacher_topk: logits of one stretch of rows
+    float *tk_logits = nullptr;
+    size_t tk_cap = 0;
 };
 
 ModelCtx *model_ctx(const GPT *m);  // nullptr (and ERR_STATE recorded) if unknown

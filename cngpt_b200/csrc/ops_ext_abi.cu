@@ -11,11 +11,8 @@ extern "C" {
 #include "cngpt_cuda.h"
 }
 
-using namespace cg;
+namespace cg {
 
-namespace {
-
-// a 4-byte aligned pointer to memory that kernels on the current device read
 int dev_ptr(const char *fn, const char *name, const void *p) {
     if (!p) {
         set_last_error(ERR_ARG, "%s: %s is NULL", fn, name);
@@ -42,6 +39,12 @@ int dev_ptr(const char *fn, const char *name, const void *p) {
     }
     return OK;
 }
+
+}  // namespace cg
+
+using namespace cg;
+
+namespace {
 
 int opt_ptr(const char *fn, const char *name, const void *p) { return p ? dev_ptr(fn, name, p) : OK; }
 
@@ -73,8 +76,8 @@ extern "C" int cngpt_cuda_sample(const float *logits, long ld, int rows, int voc
     CG_TRY(dev_ptr(fn, "u", u));
     CG_TRY(dev_ptr(fn, "tokens", tokens));
     CG_TRY(opt_ptr(fn, "logprob", logprob));
-    return sample_rows(logits, ld, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, logprob, nullptr,
-                       g_stream);
+    SampleRows a{logits, ld, rows, vocab, temperature, top_k, top_p, min_p, u, tokens, logprob};
+    return sample_rows(a, g_stream);
 }
 
 extern "C" int cngpt_cuda_topk(const float *logits, long ld, int rows, int vocab, int k, float *values,

@@ -52,7 +52,18 @@ prefix_attn_kernel(PrefixAttn a) {
     }
 }
 
+__global__ void shared_advance_kernel(int *ctr, int *suffix_len, int n) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) suffix_len[i] += 1;
+    if (threadIdx.x < 3) ctr[threadIdx.x] += 1;
+}
+
 }  // namespace
+
+int shared_advance(int *ctr, int *suffix_len, int n, cudaStream_t s) {
+    shared_advance_kernel<<<1, 256, 0, s>>>(ctr, suffix_len, n);
+    LAUNCH_CHECK();
+    return OK;
+}
 
 size_t prefix_attention_ws_bytes(int, int, int, int, int, int) { return 0; }
 

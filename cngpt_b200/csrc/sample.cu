@@ -59,19 +59,23 @@ __device__ int nth_at_key(const Row &r, uint32_t key, int m, int *shi) {
 }
 
 __global__ void __launch_bounds__(NT)
-sample_kernel(const float *__restrict__ logits, long ldl, int V, const float *__restrict__ temperature,
-              const int *__restrict__ top_k, const float *__restrict__ top_p, const float *__restrict__ min_p,
-              const float *__restrict__ u, int *__restrict__ tokens, float *__restrict__ logprob,
-              int *__restrict__ next) {
+sample_kernel(SampleRows a) {
     __shared__ double shd[NT / 32];
     __shared__ int shi[NT / 32];
     __shared__ unsigned long long best;
     __shared__ double part[NT];
     const long row = blockIdx.x;
     Row r;
-    r.x = logits + row * ldl;
+    const int V = a.V;
+    const long at = a.step ? (long)*a.step * a.rows + row : row;
+    auto put = [&](int tok, float lp) {
+        a.tokens[at] = tok;
+        if (a.next) a.next[row] = max(tok, 0);
+        if (a.logprob) a.logprob[row] = lp;
+    };
+    r.x = a.logits + row * a.ldl;
     r.V = V;
-    const float T = temperature ? temperature[row] : 1.0f;
+    const float T = a.temperature ? a.temperature[row] : 1.0f;
     r.t = (double)T;
     if (threadIdx.x == 0) best = 0;
     __syncthreads();
@@ -82,20 +86,18 @@ sample_kernel(const float *__restrict__ logits, long ldl, int V, const float *__
     __syncthreads();
     const uint32_t bk = (uint32_t)(best >> 32);
     const int bi = (int)(0xFFFFFFFFu - (uint32_t)best);
-    float p = top_p ? top_p[row] : 1.0f;
+    float p = a.top_p ? a.top_p[row] : 1.0f;
     if (bk <= RANK_NEG_INF || !(T > 0.0f) || p <= 0.0f) {
         if (threadIdx.x == 0) {
-            const bool none = bk <= RANK_NEG_INF;
-            tokens[row] = none ? -1 : bi;
-            if (next) next[row] = none ? 0 : bi;
-            if (logprob) logprob[row] = none ? -INFINITY : 0.0f;
+            if (bk <= RANK_NEG_INF) put(-1, -INFINITY);
+            else put(bi, 0.0f);
         }
         return;
     }
     r.mx = rank_value(bk);
     r.key = RANK_NEG_INF;
     r.cut = -1;
-    const int k = top_k ? top_k[row] : 0;
+    const int k = a.top_k ? a.top_k[row] : 0;
     if (k > 0 && k < V) {
         // the lowest key that fewer than k keys exceed: the k-th largest
         uint32_t lo = RANK_NEG_INF, hi = 0xFFFFFFFFu;
@@ -143,7 +145,7 @@ sample_kernel(const float *__restrict__ logits, long ldl, int V, const float *__
             }
         }
     }
-    const float mp = min_p ? min_p[row] : 0.0f;
+    const float mp = a.min_p ? a.min_p[row] : 0.0f;
     const double floor_w = mp > 0.0f ? (double)fminf(1.0f, mp) : 0.0;  // NaN: off
     auto drawn = [&](int i) {
         const uint32_t kk = rank_key(r.x[i]);
@@ -160,7 +162,7 @@ sample_kernel(const float *__restrict__ logits, long ldl, int V, const float *__
     if (threadIdx.x != 0) return;
     double total = 0.0;
     for (int t = 0; t < NT; ++t) total += part[t];
-    const double target = (double)u[row] * total;
+    const double target = (double)a.u[at] * total;
     double c = 0.0;
     int tok = bi;
     double wt = 1.0;
@@ -183,18 +185,14 @@ sample_kernel(const float *__restrict__ logits, long ldl, int V, const float *__
         if (hit) break;
         c += part[t];
     }
-    tokens[row] = tok;
-    if (next) next[row] = tok;
-    if (logprob) logprob[row] = (float)log(wt / total);
+    put(tok, (float)log(wt / total));
 }
 
 }  // namespace
 
-int sample_rows(const float *logits, long ldl, int rows, int V, const float *temperature, const int *top_k,
-                const float *top_p, const float *min_p, const float *u, int *tokens, float *logprob, int *next,
-                cudaStream_t s) {
-    if (rows <= 0) return OK;
-    sample_kernel<<<rows, NT, 0, s>>>(logits, ldl, V, temperature, top_k, top_p, min_p, u, tokens, logprob, next);
+int sample_rows(const SampleRows &a, cudaStream_t s) {
+    if (a.rows <= 0) return OK;
+    sample_kernel<<<a.rows, NT, 0, s>>>(a);
     LAUNCH_CHECK();
     return OK;
 }

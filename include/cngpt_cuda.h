@@ -205,6 +205,15 @@ int cngpt_cuda_train_step(GPT *m, const int *tokens, const int *targets, int B, 
                           float grad_clip, float *loss_out);
 int cngpt_cuda_last_loss(GPT *m, float *loss_out);
 
+/* The same step against a teacher (cngpt_cuda_distill with scale 1 / (B T) in
+ * the place of the cross-entropy): top_val / top_idx [B*T, k] are device
+ * pointers, e.g. from cngpt_cuda_teacher_topk; targets (host or device) may be
+ * NULL when alpha == 1, and entries outside [0, vocab) have no hard part. Data
+ * parallel, dropout and loss_out as in cngpt_cuda_train_step. */
+int cngpt_cuda_distill_step(GPT *m, const int *tokens, const int *targets, const float *top_val,
+                            const int *top_idx, int k, float temperature, float alpha, int B, int T, float lr,
+                            float beta1, float beta2, float eps, float wd, float grad_clip, float *loss_out);
+
 /* Decode steps of up to 8 sequences (head size 64) as one cooperative launch
  * per token - every layer, the LM head and the greedy pick, phases separated
  * by bounded grid barriers - instead of a chain of five kernels per layer.
@@ -257,6 +266,28 @@ int cngpt_cuda_load_checkpoint(GPT *m, const char *path);
  * T + n_new must not exceed block_size. */
 int cngpt_cuda_generate(GPT *m, FastCtx *f, const int *prompt, int B, int T, int n_new,
                         int *out_tokens);
+
+/* ---- sampled continuations of one prompt ---------------------------------------
+ * n_seq sequences continue the same prompt (the reference's gpt_sample,
+ * src/model.c:991-1016, runs one sequence, one host draw at a time). The prompt
+ * is prefilled once; its K and V are shared by all sequences
+ * (cngpt_cuda_prefix_attention) and every token is drawn on the device
+ * (cngpt_cuda_sample with these parameters for every sequence).
+ * prompt: host or device int[T]; u: host or device float[n_new * n_seq], step i
+ * of sequence q uses u[i * n_seq + q]; out_tokens: host int[n_seq * n_new],
+ * sequence q's tokens at q * n_new. T + n_new - 1 must not exceed block_size,
+ * n_seq not 4096. A token of -1 (no finite logit) is fed back as 0. */
+int cngpt_cuda_generate_shared(GPT *m, FastCtx *f, const int *prompt, int T, int n_seq, int n_new,
+                               float temperature, int top_k, float top_p, float min_p, const float *u,
+                               int *out_tokens);
+
+/* ---- a teacher's top logits ------------------------------------------------------
+ * The k largest logits of every position of tokens [B, T] (host or device):
+ * values / indices [B*T, k] (device), as cngpt_cuda_topk orders them. Runs the
+ * inference forward and the LM head a stretch of rows at a time, so the logits
+ * [B*T, vocab] are never stored. */
+int cngpt_cuda_teacher_topk(GPT *m, FastCtx *f, const int *tokens, int B, int T, int k, float *values,
+                            int *indices);
 
 /* ---- data-parallel training over NCCL -------------------------------------
  * One process per GPU. Rank 0 creates the id and shares it out of band. After
