@@ -137,7 +137,8 @@ extern "C" int cngpt_cuda_distill(const float *logits, long ld, int rows, int vo
 
 namespace {
 int prefix_shape(int B, int H, int Hk, int hs, int P, int S) {
-    if (B < 0 || H < 1 || Hk < 1 || H % Hk != 0 || hs < 1 || hs > 256 || P < 0 || S < 0 || (long)B * H > (1L << 30)) {
+    if (B < 0 || H < 1 || Hk < 1 || H % Hk != 0 || hs < 1 || hs > 256 || P < 0 || P > (1 << 30) || S < 0 ||
+        S > (1 << 30) || (long)B * H > (1L << 30)) {
         set_last_error(ERR_ARG, "prefix_attention: bad shape B=%d n_head=%d n_kv_head=%d hs=%d prefix=%d suffix=%d", B, H,
                        Hk, hs, P, S);
         return ERR_ARG;

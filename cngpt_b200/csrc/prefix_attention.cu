@@ -1,5 +1,22 @@
 // prefix_attention.cu - decode attention of sequences that share a prefix
 // (cngpt_cuda_prefix_attention).
+//
+// out = softmax(scale q K^T) V over the prefix's and the sequence's own keys.
+// For a set of keys the triple (m, l, o) = (max s, sum 2^(s - m), sum 2^(s - m) v)
+// with s = scale log2(e) q.k is enough: triples of disjoint sets join by
+// rescaling to the larger m. Three kernels form and join them:
+//
+//   prefix_part_kernel  all B * (n_head / n_kv_head) queries of a key/value head
+//                       against a stretch of the prefix, on the tensor cores:
+//                       the prefix is read once for all of them;
+//   suffix_part_kernel  a sequence's own queries against a stretch of its own
+//                       keys, on the CUDA cores: every key is used by one
+//                       sequence only, so its bytes set the time;
+//   join_kernel         a query's triples, in the order of the stretches.
+//
+// The three are chained by programmatic dependent launch, so the suffix blocks
+// fill the SMs that the prefix blocks leave.
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
@@ -10,51 +27,518 @@ namespace {
 
 #define LAUNCH_CHECK() do { ++g_launch_count; CG_CUDA(cudaGetLastError()); } while (0)
 
-// One warp per (sequence, head), keys in order, the softmax's running maximum
-// and sum in registers; lane l holds dimensions l, l + 32, ...
-__global__ void __launch_bounds__(128)
-prefix_attn_kernel(PrefixAttn a) {
-    const long w = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (w >= (long)a.B * a.H) return;
-    const long b = w / a.H;
-    const int h = (int)(w % a.H), hk = h / (a.H / a.Hk);
-    float q[8], o[8] = {};
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo in two tf32 numbers: hi is x rounded to 11 significant bits (half
+// away from zero, on the bit pattern), lo the exact rest, rounded the same way
+// by the tensor core's cut of the added half step. The pair is x to 2^-23.
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const float *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
+}
+
+__device__ __forceinline__ void cp_async16(float *dst, const float *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(float *dst, const float *src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+
+struct Parts {  // the triples, [stretch][B * H]
+    float *o;     // [hs] each
+    float2 *ml;
+    int n_pre, chunk;      // prefix stretches and their keys
+    int n_suf, suf_chunk;  // suffix stretches (of the capacity) and their keys
+};
+
+// ------------------------------------------------------------------ prefix
+constexpr int TK = 64;       // keys of a tile
+constexpr int PWARPS = 8;
+
+template <int HSP>
+struct PrefixCfg {
+    static constexpr int LDK = HSP + 4;  // pitches without bank conflicts for ldmatrix rows and
+    static constexpr int LDV = HSP + 8;  // for column-wise reads of four rows
+    static constexpr int STAGE = TK * (LDK + LDV);
+    static constexpr int STAGES = HSP <= 64 ? 4 : HSP <= 128 ? 2 : 1;
+};
+
+// Block: 16 RG query rows of a key/value head against `chunk` keys. Warp (rg, kg)
+// takes rows 16 rg .. 16 rg + 15 and the keys [KW kg, KW kg + KW) of every tile,
+// with its own running maximum, so warps meet only where tiles are exchanged.
+// Products are split in three (lo*hi + hi*lo + hi*hi); the small two have their
+// own accumulator, and P V starts a fresh accumulator in every tile that is
+// added in fp32, since the tensor core truncates as it accumulates.
+template <int HSP, int RG, bool SPLIT>
+__global__ void __launch_bounds__(PWARPS * 32, 1)
+prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
+    using Cfg = PrefixCfg<HSP>;
+    constexpr int KG = PWARPS / RG, KW = TK / KG, NK = KW / 8, KK = HSP / 8, ND = HSP / 8;
+    constexpr int NT = PWARPS * 32;
+    extern __shared__ float sm[];
+    pdl_trigger();
+    const int split = blockIdx.x % w.n_pre, tile = blockIdx.x / w.n_pre % n_tiles, hk = blockIdx.x / w.n_pre / n_tiles;
+    const int G = a.H / a.Hk, R = a.B * G, hs = a.hs;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rg = warp % RG, kg = warp / RG;
+    const int k_lo = split * w.chunk, k_hi = min(a.P, k_lo + w.chunk);
+    const int tiles = (k_hi - k_lo + TK - 1) / TK;
+    const float *kbase = a.pk + (long)hk * hs, *vbase = a.pv + (long)hk * hs;
+
+    auto load = [&](int i) {
+        float *dk = sm + (i % Cfg::STAGES) * Cfg::STAGE, *dv = dk + TK * Cfg::LDK;
+        const int k0 = k_lo + i * TK;
+        if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        q[i] = d < a.hs ? a.q[b * a.ldq + (long)h * a.hs + d] * a.scale : 0.0f;
+            for (int c = 0; c < TK * (HSP / 4) / NT; ++c) {
+                const int e = c * NT + threadIdx.x, r = e / (HSP / 4), d = e % (HSP / 4) * 4;
+                const bool ok = k0 + r < k_hi && d < hs;
+                const long at = ok ? (long)(k0 + r) * a.ldp + d : 0;
+                cp_async16(dk + r * Cfg::LDK + d, kbase + at, ok);
+                cp_async16(dv + r * Cfg::LDV + d, vbase + at, ok);
+            }
+        } else {
+            for (int e = threadIdx.x; e < TK * HSP; e += NT) {
+                const int r = e / HSP, d = e % HSP;
+                const bool ok = k0 + r < k_hi && d < hs;
+                const long at = ok ? (long)(k0 + r) * a.ldp + d : 0;
+                cp_async4(dk + r * Cfg::LDK + d, kbase + at, ok);
+                cp_async4(dv + r * Cfg::LDV + d, vbase + at, ok);
+            }
+        }
+    };
+    constexpr int AHEAD = Cfg::STAGES > 1 ? Cfg::STAGES - 1 : 1;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        if (i < tiles) load(i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    float m = -INFINITY, l = 0.0f;
-    const int S = a.S > 0 ? min(max(a.suffix_len[b], 0), a.S) : 0;
-    for (long j = 0; j < (long)a.P + S; ++j) {
-        const bool pre = j < a.P;
-        const long at = (pre ? j * a.ldp : b * a.seq_stride + (j - a.P) * a.lds) + (long)hk * a.hs;
-        const float *kr = (pre ? a.pk : a.sk) + at, *vr = (pre ? a.pv : a.sv) + at;
-        float s = 0.0f;
+
+    // the rows' fragments of Q scale log2(e), split, in registers
+    uint32_t qh[KK][4], ql[KK][4];
+    {
+        const float sc = a.scale * LOG2E;
+        const int r0 = tile * 16 * RG + rg * 16 + g, r1 = r0 + 8;
+        auto row = [&](int r) { return a.q + (long)(r / G) * a.ldq + (long)(hk * G + r % G) * hs; };
+        const float *p0 = row(min(r0, R - 1)), *p1 = row(min(r1, R - 1));
+#pragma unroll
+        for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 8 * k + t + (e >> 1) * 4;
+                const bool ok = d < hs && ((e & 1) ? r1 : r0) < R;
+                const float v = ok ? ((e & 1) ? p1 : p0)[d] * sc : 0.0f;
+                if constexpr (SPLIT) split_tf32(v, qh[k][e], ql[k][e]);
+                else qh[k][e] = __float_as_uint(v);
+            }
+    }
+
+    float o[ND][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int i = 0; i < tiles; ++i) {
+        if constexpr (Cfg::STAGES > 1) asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // tile i is there, and every warp is done with tile i - 1
+        if constexpr (Cfg::STAGES > 1) {
+            if (i + AHEAD < tiles) load(i + AHEAD);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        const float *sk = sm + (i % Cfg::STAGES) * Cfg::STAGE, *sv = sk + TK * Cfg::LDK;
+        const int valid = min(TK, k_hi - k_lo - i * TK);
+        if (kg * KW < valid) {
+            float s[NK][4] = {}, sl[NK][4] = {};
+            // accumulator column n of a group of 8 holds key (n >> 1) + 4 (n & 1),
+            // so that a thread's two columns are the keys t and t + 4 of the A
+            // fragment that the same registers form in P V
+            const float *kr = sk + (kg * KW + ((lane & 7) >> 1) + 4 * (lane & 1)) * Cfg::LDK + (lane >> 3) * 4;
+#pragma unroll
+            for (int k = 0; k < KK; k += 2) {
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    uint32_t b[4];
+                    ldsm4(b, kr + j * 8 * Cfg::LDK + k * 8);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if constexpr (SPLIT) {
+                            uint32_t h0, h1, l0, l1;
+                            split_tf32(__uint_as_float(b[2 * u]), h0, l0);
+                            split_tf32(__uint_as_float(b[2 * u + 1]), h1, l1);
+                            mma8(sl[j], ql[k + u], h0, h1);
+                            mma8(sl[j], qh[k + u], l0, l1);
+                            mma8(s[j], qh[k + u], h0, h1);
+                        } else {
+                            mma8(s[j], qh[k + u], b[2 * u], b[2 * u + 1]);
+                        }
+                    }
+                }
+            }
+            float mx[2] = {m[0], m[1]};
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = kg * KW + j * 8 + t + (e & 1) * 4;
+                    s[j][e] = key < valid ? s[j][e] + sl[j][e] : -INFINITY;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
+                }
+            float c[2], ref[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                ref[r] = mx[r] == -INFINITY ? 0.0f : mx[r];
+                c[r] = ex2(m[r] - ref[r]);
+                m[r] = mx[r];
+                l[r] *= c[r];
+            }
+            uint32_t ph[NK][4], pl[NK][4];
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = ex2(s[j][e] - ref[e >> 1]);
+                    l[e >> 1] += p;
+                    const int x = (e >> 1) + 2 * (e & 1);  // C fragment {0,1,2,3} -> A fragment {0,2,1,3}
+                    if constexpr (SPLIT) split_tf32(p, ph[j][x], pl[j][x]);
+                    else ph[j][x] = __float_as_uint(p);
+                }
+            const float *vr = sv + (kg * KW + t) * Cfg::LDV + g;
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                float acc[4] = {}, acl[4] = {};
+#pragma unroll
+                for (int j = 0; j < NK; ++j) {
+                    const float v0 = vr[j * 8 * Cfg::LDV + n * 8], v1 = vr[(j * 8 + 4) * Cfg::LDV + n * 8];
+                    if constexpr (SPLIT) {
+                        uint32_t h0, h1, l0, l1;
+                        split_tf32(v0, h0, l0);
+                        split_tf32(v1, h1, l1);
+                        mma8(acl, pl[j], h0, h1);
+                        mma8(acl, ph[j], l0, l1);
+                        mma8(acc, ph[j], h0, h1);
+                    } else {
+                        mma8(acc, ph[j], __float_as_uint(v0), __float_as_uint(v1));
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][e] = fmaf(o[n][e], c[e >> 1], acc[e] + acl[e]);
+            }
+        }
+        if constexpr (Cfg::STAGES == 1) {
+            __syncthreads();
+            if (i + 1 < tiles) load(i + 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+
+    // join the KG warps of a row group, in their order
+    float *so = sm;                                       // [KG][16 RG][HSP]
+    float2 *sml = (float2 *)(so + KG * 16 * RG * HSP);    // [KG][16 RG]
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        const int rr = rg * 16 + g + 8 * r;
+        if (t == 0) sml[kg * 16 * RG + rr] = make_float2(m[r], l[r]);
+#pragma unroll
+        for (int n = 0; n < ND; ++n)
+            *(float2 *)(so + (kg * 16 * RG + rr) * HSP + n * 8 + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    }
+    __syncthreads();
+    const long BH = (long)a.B * a.H;
+    for (int e = threadIdx.x; e < 16 * RG * HSP; e += NT) {
+        const int rr = e / HSP, d = e % HSP, r = tile * 16 * RG + rr;
+        if (r >= R) continue;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KG; ++k) mm = fmaxf(mm, sml[k * 16 * RG + rr].x);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float ll = 0.0f, oo = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KG; ++k) {
+            const float2 p = sml[k * 16 * RG + rr];
+            const float f = ex2(p.x - ref);
+            ll = fmaf(p.y, f, ll);
+            oo = fmaf(so[(k * 16 * RG + rr) * HSP + d], f, oo);
+        }
+        const long id = split * BH + (long)(r / G) * a.H + hk * G + r % G;
+        if (d < hs) w.o[id * hs + d] = oo;
+        if (d == 0) w.ml[id] = make_float2(mm, ll);
+    }
+}
+
+// ------------------------------------------------------------------ suffix
+// Block: one sequence, one key/value head, one stretch of CH keys. LPK lanes hold
+// one key's row (NF float4 each), so a warp reads 32 / LPK whole rows at a time;
+// all K and V rows of the stretch are on their way before the first is used.
+constexpr int SWARPS = 8;
+
+template <int LPK, int NF>
+struct SuffixCfg {
+    static constexpr int KPI = 32 / LPK, ITER = 8 / NF, CH = SWARPS * KPI * ITER;
+};
+
+__device__ __forceinline__ float4 row4(const float *p, int d, int hs, bool ok, bool vec) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (!ok) return v;
+    if (vec) {
+        if (d < hs) v = *(const float4 *)(p + d);
+    } else {
+        if (d < hs) v.x = p[d];
+        if (d + 1 < hs) v.y = p[d + 1];
+        if (d + 2 < hs) v.z = p[d + 2];
+        if (d + 3 < hs) v.w = p[d + 3];
+    }
+    return v;
+}
+
+template <int LPK, int NF>
+__global__ void __launch_bounds__(SWARPS * 32)
+suffix_part_kernel(PrefixAttn a, Parts w, bool vec) {
+    using Cfg = SuffixCfg<LPK, NF>;
+    __shared__ float so[SWARPS][LPK * 4 * NF];
+    __shared__ float2 sml[SWARPS];
+    pdl_trigger();
+    const int chunk = blockIdx.x % w.n_suf, hk = blockIdx.x / w.n_suf % a.Hk, b = blockIdx.x / w.n_suf / a.Hk;
+    const int len = min(max(a.suffix_len[b], 0), a.S), j0 = chunk * Cfg::CH;
+    if (j0 < len) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPK, li = lane % LPK;
+        const int G = a.H / a.Hk, hs = a.hs;
+        const float *kb = a.sk + b * a.seq_stride + (long)hk * hs, *vb = a.sv + b * a.seq_stride + (long)hk * hs;
+        float4 k[Cfg::ITER][NF], v[Cfg::ITER][NF];
+#pragma unroll
+        for (int i = 0; i < Cfg::ITER; ++i) {
+            const int j = j0 + (i * SWARPS + warp) * Cfg::KPI + sub;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) k[i][f] = row4(kb + (long)j * a.lds, (li + f * LPK) * 4, hs, j < len, vec);
+        }
+#pragma unroll
+        for (int i = 0; i < Cfg::ITER; ++i) {
+            const int j = j0 + (i * SWARPS + warp) * Cfg::KPI + sub;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) v[i][f] = row4(vb + (long)j * a.lds, (li + f * LPK) * 4, hs, j < len, vec);
+        }
+        const float sc = a.scale * LOG2E;
+        for (int gq = 0; gq < G; ++gq) {
+            const float *qr = a.q + b * a.ldq + (long)(hk * G + gq) * hs;
+            float s[Cfg::ITER] = {}, m = -INFINITY;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const float4 q = row4(qr, (li + f * LPK) * 4, hs, true, false);
+#pragma unroll
+                for (int i = 0; i < Cfg::ITER; ++i)
+                    s[i] = fmaf(q.x, k[i][f].x, fmaf(q.y, k[i][f].y, fmaf(q.z, k[i][f].z, fmaf(q.w, k[i][f].w, s[i]))));
+            }
+#pragma unroll
+            for (int i = 0; i < Cfg::ITER; ++i) {
+#pragma unroll
+                for (int x = LPK / 2; x > 0; x >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
+                const int j = j0 + (i * SWARPS + warp) * Cfg::KPI + sub;
+                s[i] = j < len ? s[i] * sc : -INFINITY;
+                m = fmaxf(m, s[i]);
+            }
+#pragma unroll
+            for (int x = LPK; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f;
+            float4 o[NF];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) o[f] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < Cfg::ITER; ++i) {
+                const float p = ex2(s[i] - ref);
+                l += p;
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    o[f].x = fmaf(p, v[i][f].x, o[f].x);
+                    o[f].y = fmaf(p, v[i][f].y, o[f].y);
+                    o[f].z = fmaf(p, v[i][f].z, o[f].z);
+                    o[f].w = fmaf(p, v[i][f].w, o[f].w);
+                }
+            }
+#pragma unroll
+            for (int x = LPK; x < 32; x <<= 1) {
+                l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    o[f].x += __shfl_xor_sync(0xffffffffu, o[f].x, x);
+                    o[f].y += __shfl_xor_sync(0xffffffffu, o[f].y, x);
+                    o[f].z += __shfl_xor_sync(0xffffffffu, o[f].z, x);
+                    o[f].w += __shfl_xor_sync(0xffffffffu, o[f].w, x);
+                }
+            }
+            if (gq) __syncthreads();  // the head before has been read
+            if (lane == 0) sml[warp] = make_float2(m, l);
+            if (sub == 0)
+#pragma unroll
+                for (int f = 0; f < NF; ++f) *(float4 *)&so[warp][(li + f * LPK) * 4] = o[f];
+            __syncthreads();
+            const long id = (long)(w.n_pre + chunk) * a.B * a.H + (long)b * a.H + hk * G + gq;
+            float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+            for (int x = 0; x < SWARPS; ++x) mm = fmaxf(mm, sml[x].x);
+            const float r2 = mm == -INFINITY ? 0.0f : mm;
+            for (int d = threadIdx.x; d < hs; d += SWARPS * 32) {
+                float oo = 0.0f;
+#pragma unroll
+                for (int x = 0; x < SWARPS; ++x) oo = fmaf(so[x][d], ex2(sml[x].x - r2), oo);
+                w.o[id * hs + d] = oo;
+            }
+            if (threadIdx.x == 0) {
+#pragma unroll
+                for (int x = 0; x < SWARPS; ++x) ll = fmaf(sml[x].y, ex2(sml[x].x - r2), ll);
+                w.ml[id] = make_float2(mm, ll);
+            }
+        }
+    }
+    pdl_wait();  // the prefix blocks: the kernel that waits for this one waits for them too
+}
+
+// -------------------------------------------------------------------- join
+constexpr int JWARPS = 4;
+
+__global__ void __launch_bounds__(JWARPS * 32)
+join_kernel(PrefixAttn a, Parts w) {
+    __shared__ float so[JWARPS][256];
+    __shared__ float sl[JWARPS];
+    const long row = blockIdx.x, BH = (long)a.B * a.H;
+    const int b = (int)(row / a.H), h = (int)(row % a.H), hs = a.hs;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int len = a.S > 0 ? min(max(a.suffix_len[b], 0), a.S) : 0;
+    const int n = w.n_pre + (len > 0 ? (len + w.suf_chunk - 1) / w.suf_chunk : 0);
+    pdl_wait();
+    float m = -INFINITY;
+    for (int s = lane; s < n; s += 32) m = fmaxf(m, w.ml[s * BH + row].x);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    // each warp joins every JWARPS-th stretch
+    float l = 0.0f, o[8] = {};
+    for (int s = warp; s < n; s += JWARPS) {
+        const float2 p = w.ml[s * BH + row];
+        const float f = ex2(p.x - ref);
+        l = fmaf(p.y, f, l);
+        const float *po = w.o + (s * BH + row) * hs;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < a.hs) s = fmaf(q[i], kr[lane + 32 * i], s);
-        s = warp_sum(s);
-        if (s == -INFINITY) continue;
-        const float mn = fmaxf(m, s), c = expf(m - mn), p = expf(s - mn);
-        l = l * c + p;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < a.hs) o[i] = fmaf(p, vr[lane + 32 * i], o[i] * c);
+            if (lane + 32 * i < hs) o[i] = fmaf(po[lane + 32 * i], f, o[i]);
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        if (d < a.hs) a.out[b * a.ldo + (long)h * a.hs + d] = o[i] * inv;
+    for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < hs) so[warp][lane + 32 * i] = o[i];
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    l = sl[0];
+#pragma unroll
+    for (int x = 1; x < JWARPS; ++x) l += sl[x];
+    const float inv = n > 0 ? 1.0f / l : 0.0f;
+    for (int d = threadIdx.x; d < hs; d += JWARPS * 32) {
+        float oo = so[0][d];
+#pragma unroll
+        for (int x = 1; x < JWARPS; ++x) oo += so[x][d];
+        a.out[b * a.ldo + (long)h * hs + d] = n > 0 ? oo * inv : 0.0f;
     }
 }
 
 __global__ void shared_advance_kernel(int *ctr, int *suffix_len, int n) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) suffix_len[i] += 1;
     if (threadIdx.x < 3) ctr[threadIdx.x] += 1;
+}
+
+// ------------------------------------------------------------- the launches
+int row_groups(long R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+
+// Stretches: the prefix is cut so that its blocks fill the SMs about once (one
+// block an SM), but not below one tile; the suffixes into what one block loads
+// at once.
+Parts plan(int B, int H, int Hk, int hs, int P, int S) {
+    Parts w{};
+    const long R = (long)B * (H / Hk);
+    const int rg = row_groups(R);
+    if (P > 0) {
+        const long n_tiles = (R + 16 * rg - 1) / (16 * rg), tiles = (P + TK - 1) / TK;
+        const long want = std::max<long>(1, 148 / std::max<long>(1, Hk * n_tiles));
+        const long per = (tiles + std::min(want, tiles) - 1) / std::min(want, tiles);
+        w.chunk = (int)(per * TK);
+        w.n_pre = (int)((P + (long)w.chunk - 1) / w.chunk);
+    }
+    w.suf_chunk = hs <= 32 ? SuffixCfg<8, 1>::CH : hs <= 64 ? SuffixCfg<16, 1>::CH
+                : hs <= 128 ? SuffixCfg<32, 1>::CH : SuffixCfg<32, 2>::CH;
+    w.n_suf = (int)(((long)S + w.suf_chunk - 1) / w.suf_chunk);
+    return w;
+}
+
+template <class K, class... A>
+int launch_pdl(K kernel, long grid, int threads, size_t smem, bool chained, cudaStream_t s, A... args) {
+    if (grid > 0x7FFFFFFFL) {
+        set_last_error(ERR_ARG, "prefix_attention: %ld blocks are too many", grid);
+        return ERR_ARG;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = chained ? 1 : 0;
+    CG_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    ++g_launch_count;
+    return OK;
+}
+
+template <int HSP, int RG, bool SPLIT>
+int launch_prefix(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
+    using Cfg = PrefixCfg<HSP>;
+    constexpr size_t join = (size_t)(PWARPS / RG) * 16 * RG * (HSP + 2);
+    constexpr size_t smem = std::max((size_t)Cfg::STAGES * Cfg::STAGE, join) * sizeof(float);
+    static bool set = false;
+    if (!set) {
+        CG_CUDA(cudaFuncSetAttribute(prefix_part_kernel<HSP, RG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)smem));
+        set = true;
+    }
+    const long R = (long)a.B * (a.H / a.Hk), n_tiles = (R + 16 * RG - 1) / (16 * RG);
+    const bool vec = a.hs % 4 == 0 && a.ldp % 4 == 0 && ((uintptr_t)a.pk | (uintptr_t)a.pv) % 16 == 0;
+    return launch_pdl(prefix_part_kernel<HSP, RG, SPLIT>, (long)w.n_pre * n_tiles * a.Hk, PWARPS * 32, smem, false, s, a, w,
+                      (int)n_tiles, vec);
+}
+
+template <int HSP, bool SPLIT>
+int dispatch_rows(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
+    const int rg = row_groups((long)a.B * (a.H / a.Hk));
+    if (rg == 1) return launch_prefix<HSP, 1, SPLIT>(a, w, s);
+    if (rg == 2) return launch_prefix<HSP, 2, SPLIT>(a, w, s);
+    return launch_prefix<HSP, 4, SPLIT>(a, w, s);
+}
+
+template <bool SPLIT>
+int dispatch_hs(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
+    if (a.hs <= 32) return dispatch_rows<32, SPLIT>(a, w, s);
+    if (a.hs <= 64) return dispatch_rows<64, SPLIT>(a, w, s);
+    if (a.hs <= 96) return dispatch_rows<96, SPLIT>(a, w, s);
+    if (a.hs <= 128) return dispatch_rows<128, SPLIT>(a, w, s);
+    return dispatch_rows<256, SPLIT>(a, w, s);
 }
 
 }  // namespace
@@ -65,14 +549,35 @@ int shared_advance(int *ctr, int *suffix_len, int n, cudaStream_t s) {
     return OK;
 }
 
-size_t prefix_attention_ws_bytes(int, int, int, int, int, int) { return 0; }
+size_t prefix_attention_ws_bytes(int B, int H, int Hk, int hs, int P, int S) {
+    const Parts w = plan(B, H, Hk, hs, P, S);
+    const size_t rows = (size_t)(w.n_pre + w.n_suf) * B * H;
+    return (rows * hs * sizeof(float) + 15) / 16 * 16 + rows * sizeof(float2);
+}
 
-int prefix_attention(const PrefixAttn &a, void *, cudaStream_t s) {
+int prefix_attention(const PrefixAttn &a, void *ws, cudaStream_t s) {
     if (a.B <= 0) return OK;
-    const long warps = (long)a.B * a.H;
-    prefix_attn_kernel<<<(unsigned)((warps + 3) / 4), 128, 0, s>>>(a);
-    LAUNCH_CHECK();
-    return OK;
+    Parts w = plan(a.B, a.H, a.Hk, a.hs, a.P, a.S);
+    w.o = (float *)ws;
+    const size_t rows = (size_t)(w.n_pre + w.n_suf) * a.B * a.H;
+    w.ml = (float2 *)((char *)ws + (rows * a.hs * sizeof(float) + 15) / 16 * 16);
+    bool chained = false;
+    if (w.n_pre > 0) {
+        CG_TRY(precision() == PREC_TF32 ? dispatch_hs<false>(a, w, s) : dispatch_hs<true>(a, w, s));
+        chained = true;
+    }
+    if (w.n_suf > 0) {
+        const bool vec = a.hs % 4 == 0 && a.lds % 4 == 0 && a.seq_stride % 4 == 0 &&
+                         ((uintptr_t)a.sk | (uintptr_t)a.sv) % 16 == 0;
+        const long grid = (long)w.n_suf * a.Hk * a.B;
+        auto go = [&](auto kernel) { return launch_pdl(kernel, grid, SWARPS * 32, 0, chained, s, a, w, vec); };
+        if (a.hs <= 32) CG_TRY(go(suffix_part_kernel<8, 1>));
+        else if (a.hs <= 64) CG_TRY(go(suffix_part_kernel<16, 1>));
+        else if (a.hs <= 128) CG_TRY(go(suffix_part_kernel<32, 1>));
+        else CG_TRY(go(suffix_part_kernel<32, 2>));
+        chained = true;
+    }
+    return launch_pdl(join_kernel, (long)a.B * a.H, JWARPS * 32, 0, chained, s, a, w);
 }
 
 }  // namespace cg

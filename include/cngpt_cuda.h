@@ -180,7 +180,7 @@ int cngpt_cuda_distill(const float *logits, long ld, int rows, int vocab, const 
  * read once for all sequences. A sequence that sees no key gets zeros. What is
  * read has to be finite and below 1e37 in size; keys behind a sequence's suffix
  * and the gaps that the pitches leave are not read.
- * out [B, n_head, hs] (row pitch ldo). hs <= 256; 0 <= prefix_len, max_suffix;
+ * out [B, n_head, hs] (row pitch ldo). hs <= 256; 0 <= prefix_len, max_suffix <= 2^30;
  * pk / pv may be NULL when prefix_len == 0, sk / sv when max_suffix == 0 (and
  * suffix_len then too). All pointers are device pointers.
  * ws: device workspace of at least prefix_attention_workspace bytes, 16-byte
