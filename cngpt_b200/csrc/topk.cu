@@ -1,4 +1,17 @@
 // topk.cu - the k largest logits of every row in falling order (cngpt_cuda_topk).
+//
+// One pass over the row. The block keeps the k best of what it has seen as
+// 64-bit keys (ordered bits of the logit, then the inverted index, so that the
+// lower index wins among equals) and the logit `low` of the worst of them; of
+// the next chunk only logits above `low` can matter (an equal one has a higher
+// index than all k). In a row of random order the k-th best rises so fast that
+// about k (1 + log(chunks)) logits pass after the first chunk; whenever many have
+// passed, a radix selection cuts the candidates back to k. So the time is that
+// of reading the logits once, whatever k.
+#include <algorithm>
+
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "rank.cuh"
@@ -6,50 +19,244 @@
 namespace cg {
 namespace {
 
+namespace coop = cooperative_groups;
+
 #define LAUNCH_CHECK() do { ++g_launch_count; CG_CUDA(cudaGetLastError()); } while (0)
 
-constexpr int NT = 512;
+typedef unsigned long long u64;
 
-__device__ int block_count(int v, int *sh) {
+constexpr int NT = 256;              // threads
+constexpr int QUADS = 4;             // 16-byte loads of a thread and chunk
+constexpr int CHUNK = NT * QUADS * 4;
+constexpr int BINS = 2048;           // radix 2^11
+constexpr int TRIGGER = 256;         // candidates below which no selection is worth its time
+
+__device__ __forceinline__ u64 make_key(float x, uint32_t i) { return ((u64)rank_key(x) << 32) | (0xFFFFFFFFu - i); }
+
+struct Smem {
+    // hist is also where a selection collects the k it keeps (TOPK_MAX * 8 bytes)
+    union {
+        uint32_t hist[BINS];
+        u64 keep[TOPK_MAX];
+    };
+    uint32_t warp[NT / 32];
+    int count;             // candidates in the buffer
+    int bin, need, equal;  // of a selection: the bin that holds the k-th, how many of it belong, how many it has
+    int kept;
+    uint32_t low;          // rank_key of the worst one kept
+};
+
+// Cuts the n > k candidates in buf to the k largest (any order) and sets low.
+// Radix from the top: 11, 11 and 10 bits of the logit, then of the index (only
+// where equal logits straddle the cut); ends as soon as the bin that holds the
+// k-th is needed whole. hist is zero before and after.
+__device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 prefix = 0;
+    int need = k, top = 64;
+    while (true) {
+        const int bits = (top == 42 || top == 10) ? 10 : 11, shift = top - bits;
+        for (int i = tid; i < n; i += NT) {
+            const u64 key = buf[i];
+            if (top == 64 || (key >> top) == prefix) atomicAdd(&sm.hist[(uint32_t)(key >> shift) & ((1u << bits) - 1)], 1u);
+        }
+        __syncthreads();
+        // thread t sums 8 bins from the top; exclusive scan over the threads
+        const int hi = BINS - 8 * tid;
+        uint32_t c[8], s = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int j = 0; j < 8; ++j) {
+            c[j] = sm.hist[hi - 1 - j];
+            sm.hist[hi - 1 - j] = 0;
+            s += c[j];
+        }
+        uint32_t inc = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) sm.warp[warp] = inc;
+        __syncthreads();
+        uint32_t before = inc - s;
+        for (int w = 0; w < warp; ++w) before += sm.warp[w];
+        if (before < (uint32_t)need && before + s >= (uint32_t)need) {
+            uint32_t b = before;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (b < (uint32_t)need && b + c[j] >= (uint32_t)need) {
+                    sm.bin = hi - 1 - j;
+                    sm.need = need - (int)b;
+                    sm.equal = (int)c[j];
+                }
+                b += c[j];
+            }
+        }
+        __syncthreads();
+        prefix = (prefix << bits) | (u64)sm.bin;
+        need = sm.need;
+        top = shift;
+        if (sm.equal == need) break;
+    }
+    const u64 cut = prefix << top;
+    if (tid == 0) {
+        sm.kept = 0;
+        sm.low = 0xFFFFFFFFu;
+    }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    uint32_t low = 0xFFFFFFFFu;
+    for (int i = tid; i < n; i += NT) {
+        const u64 key = buf[i];
+        if (key >= cut) {
+            sm.keep[atomicAdd(&sm.kept, 1)] = key;
+            low = min(low, (uint32_t)(key >> 32));
+        }
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (lane == 0) atomicMin(&sm.low, low);
     __syncthreads();
-    int s = 0;
-    for (int w = 0; w < NT / 32; ++w) s += sh[w];
-    return s;
+    for (int i = tid; i < k; i += NT) buf[i] = sm.keep[i];
+    __syncthreads();
+    for (int i = tid; i < BINS; i += NT) sm.hist[i] = 0;
+    if (tid == 0) sm.count = k;
+    __syncthreads();
 }
 
-// Block per row. A token's rank is the number of 64-bit keys (logit key, index
-// inverted) above its own; the k-th largest such key is found by bisection, the
-// k tokens at or above it are collected and ordered by counting.
+// Cluster of 1 to 8 blocks per row, each with a stretch of it; block 0 then
+// joins the stretches' candidates from the others' shared memory.
 __global__ void __launch_bounds__(NT)
 topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__restrict__ values,
-            int *__restrict__ indices) {
-    __shared__ int sh[NT / 32];
-    __shared__ unsigned long long cand[TOPK_MAX];
-    __shared__ int n;
-    const float *x = logits + (long)blockIdx.x * ldl;
-    auto key = [&](int i) { return ((unsigned long long)rank_key(x[i]) << 32) | (0xFFFFFFFFu - (uint32_t)i); };
-    unsigned long long lo = 0, hi = ~0ull;
-    while (lo < hi) {
-        const unsigned long long mid = lo + (hi - lo) / 2;
-        int c = 0;
-        for (int i = threadIdx.x; i < V; i += NT) c += key(i) > mid;
-        if (block_count(c, sh) < k) hi = mid;
-        else lo = mid + 1;
+            int *__restrict__ indices, int stretch) {
+    extern __shared__ u64 buf[];  // [max(2 k, TRIGGER) + CHUNK + 8]
+    __shared__ Smem sm;
+    auto cluster = coop::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    const long row = blockIdx.x / parts;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int lo = min(V, part * stretch), hi = min(V, lo + stretch), n = hi - lo;
+    const float *x = logits + row * ldl + lo;
+    for (int i = tid; i < BINS; i += NT) sm.hist[i] = 0;
+    if (tid == 0) sm.count = 0;
+    // elements before the first 16-byte boundary, whole groups of four, the rest
+    const int head = min(n, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (n - head) / 4;
+    const float4 *x4 = (const float4 *)(x + head);
+    float4 v[QUADS], nx[QUADS];
+    auto fetch = [&](float4 *dst, int c) {
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) {
+            const int q = (c * QUADS + j) * NT + tid;
+            dst[j] = q < quads ? __ldcs(x4 + q) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    fetch(nx, 0);
+    __syncthreads();
+    if (tid < head) buf[atomicAdd(&sm.count, 1)] = make_key(x[tid], lo + tid);
+    __syncthreads();
+    const int chunks = (quads + QUADS * NT - 1) / (QUADS * NT);
+    bool all = true;     // fewer than k seen: every element is a candidate
+    float low = 0.0f;    // else those above low (any number if low is NaN)
+    bool any_number = false;
+    for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) v[j] = nx[j];
+        if (c + 1 < chunks) fetch(nx, c + 1);
+        uint32_t pass = 0;
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) {
+            const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            const bool in = (c * QUADS + j) * NT + tid < quads;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const bool p = all || (any_number ? e[y] == e[y] : e[y] > low);
+                pass |= (in && p) ? 1u << (4 * j + y) : 0u;
+            }
+        }
+        if (__any_sync(0xffffffffu, pass != 0)) {
+            const int mine = __popc(pass);
+            int inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += u;
+            }
+            int base = 0;
+            if (lane == 31) base = atomicAdd(&sm.count, inc);
+            int at = __shfl_sync(0xffffffffu, base, 31) + inc - mine;
+#pragma unroll
+            for (int j = 0; j < QUADS; ++j) {
+                const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    if (pass >> (4 * j + y) & 1)
+                        buf[at++] = make_key(e[y], (uint32_t)(lo + head + 4 * ((c * QUADS + j) * NT + tid) + y));
+            }
+        }
+        __syncthreads();
+        const int have = sm.count;
+        // the buffer holds what may stay uncut and one more chunk
+        if (have > k && (all || have >= max(2 * k, TRIGGER))) {
+            select_k(buf, have, k, sm);
+            all = false;
+            low = rank_value(sm.low);
+            any_number = sm.low == 0u;
+        } else {
+            __syncthreads();  // count has been read by all
+        }
     }
-    if (threadIdx.x == 0) n = 0;
+    {  // the last ones (their indices are the highest, so they come last)
+        const int i = head + 4 * quads + tid;
+        if (i < n && (all || (any_number ? x[i] == x[i] : x[i] > low))) buf[atomicAdd(&sm.count, 1)] = make_key(x[i], lo + i);
+        __syncthreads();
+    }
+    const int seen = sm.count;
     __syncthreads();
-    for (int i = threadIdx.x; i < V; i += NT)
-        if (key(i) >= lo) cand[atomicAdd(&n, 1)] = key(i);
+    if (seen > k) select_k(buf, seen, k, sm);
+    if (parts > 1) {
+        cluster.sync();
+        if (part == 0) {
+            int have = sm.count;
+            for (int p = 1; p < parts; ++p) {
+                const int m = *cluster.map_shared_rank(&sm.count, p);
+                const u64 *other = cluster.map_shared_rank(buf, p);
+                for (int i = tid; i < m; i += NT) buf[have + i] = other[i];
+                have += m;
+            }
+            __syncthreads();
+            if (have > k) select_k(buf, have, k, sm);
+        }
+        cluster.sync();  // the others' memory has been read
+        if (part != 0) return;
+    }
+    // order the k by counting (short lists) or by a bitonic network
+    if (k <= 128) {
+        for (int c = tid; c < k; c += NT) {
+            const u64 key = buf[c];
+            int r = 0;
+            for (int j = 0; j < k; ++j) r += buf[j] > key;
+            values[row * k + r] = rank_value((uint32_t)(key >> 32));
+            indices[row * k + r] = (int)(0xFFFFFFFFu - (uint32_t)key);
+        }
+        return;
+    }
+    int m = 256;
+    while (m < k) m <<= 1;
+    for (int i = k + tid; i < m; i += NT) buf[i] = 0;  // below every key of a token
+    for (int size = 2; size <= m; size <<= 1)
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            __syncthreads();
+            for (int i = tid; i < m / 2; i += NT) {
+                const int a = 2 * i - (i & (d - 1)), b = a + d;
+                const u64 u = buf[a], w = buf[b];
+                if ((u < w) == ((a & size) == 0)) {
+                    buf[a] = w;
+                    buf[b] = u;
+                }
+            }
+        }
     __syncthreads();
-    for (int c = threadIdx.x; c < k; c += NT) {
-        int r = 0;
-        for (int j = 0; j < k; ++j) r += cand[j] > cand[c];
-        values[(long)blockIdx.x * k + r] = rank_value((uint32_t)(cand[c] >> 32));
-        indices[(long)blockIdx.x * k + r] = (int)(0xFFFFFFFFu - (uint32_t)cand[c]);
+    for (int i = tid; i < k; i += NT) {
+        values[row * k + i] = rank_value((uint32_t)(buf[i] >> 32));
+        indices[row * k + i] = (int)(0xFFFFFFFFu - (uint32_t)buf[i]);
     }
 }
 
@@ -57,8 +264,35 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
 
 int topk_rows(const float *logits, long ldl, int rows, int V, int k, float *values, int *indices, cudaStream_t s) {
     if (rows <= 0) return OK;
-    topk_kernel<<<rows, NT, 0, s>>>(logits, ldl, V, k, values, indices);
-    LAUNCH_CHECK();
+    // Few rows leave SMs idle: cut each among up to 8 blocks, as long as a stretch
+    // is a chunk or more and the stretches' k candidates fit one block's buffer.
+    int parts = 1;
+    while (parts < 8 && (long)rows * parts * 2 <= num_sms() && V >= 2 * parts * CHUNK && 2 * parts * k <= k + CHUNK) parts *= 2;
+    const int stretch = ((V + parts - 1) / parts + 3) / 4 * 4;
+    if ((long)rows * parts > 0x7FFFFFFFL) {
+        set_last_error(ERR_ARG, "topk: %d rows are too many", rows);
+        return ERR_ARG;
+    }
+    const size_t smem = (size_t)(std::max(2 * k, TRIGGER) + CHUNK + 8) * sizeof(u64);
+    static bool set = false;
+    if (!set) {
+        CG_CUDA(cudaFuncSetAttribute(topk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)((2 * TOPK_MAX + CHUNK + 8) * sizeof(u64))));
+        set = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * parts));
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CG_CUDA(cudaLaunchKernelEx(&cfg, topk_kernel, logits, ldl, V, k, values, indices, stretch));
+    ++g_launch_count;
     return OK;
 }
 
