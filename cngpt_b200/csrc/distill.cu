@@ -1,13 +1,14 @@
 // distill.cu - loss and gradient of a student's logits against a teacher's
 // list of top logits and hard targets (cngpt_cuda_distill).
 //
-// With c = log2(e) / t, a row's softmax at temperature t needs m = max x and
-// s_t = sum 2^((x - m) c); loss and gradient then are
-//   sum p (log p - (x - m) / tau + log s_tau)  and  a 2^((x - m) c) / s_t - ...,
-// the list's and the target's entries apart. Reading a row once and writing its
-// gradient once is all that has to move (8 bytes a logit, 4 without gradient),
-// so a cluster of blocks keeps the row in its shared memory between the pass
-// that forms m and the sums and the pass that writes.
+// With c = log2(e) / t and R = max x c, a row's softmax at temperature t needs
+// s_t = sum 2^(x c - R): loss and gradient then are
+//   sum p (log p - ln2 (x c - R - log2 s_tau))  and  a 2^(x c - R) / s_t - ...,
+// the list's and the target's entries apart. R is one rounded number that both
+// passes subtract inside one fma, so its rounding cancels. Reading a row once and
+// writing its gradient once is all that has to move (8 bytes a logit, 4 without
+// gradient), so a cluster of blocks keeps the row in its shared memory between
+// the pass that forms the sums and the pass that writes.
 #include <algorithm>
 #include <cmath>
 
@@ -24,11 +25,10 @@ namespace coop = cooperative_groups;
 #define LAUNCH_CHECK() do { ++g_launch_count; CG_CUDA(cudaGetLastError()); } while (0)
 
 constexpr int NT = 256;
-constexpr int QUADS = 4;                // 16-byte loads of a thread in flight
 constexpr int MAX_PARTS = 8;
 constexpr int SLICE_BYTES = 52 * 1024;  // of a row in a block's shared memory: four blocks an SM
-constexpr int SLICE_MAX = 200 * 1024;   // where eight blocks need more than that: one block an SM
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -36,21 +36,20 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Maximum and the sums at both temperatures of a part of a row. A part of -inf
-// alone has m = -inf and sums of 0; NaN stays in the sums.
+// Maximum of a part of a row and its sums at both temperatures, relative to
+// R(m). A part of -inf alone has m = -inf and sums of 0; NaN stays in the sums.
 struct Stats {
     float m, st, s1;
 };
 
-__device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.0f : m; }
+__device__ __forceinline__ float scaled_max(float m, float c) { return m == -INFINITY ? 0.0f : __fmul_rn(m, c); }
 
-__device__ __forceinline__ Stats merge(const Stats &a, const Stats &b, float ct) {
-    Stats r;
-    r.m = fmaxf(a.m, b.m);
-    const float ref = ref_of(r.m), da = a.m - ref, db = b.m - ref;
-    r.st = a.st * ex2(da * ct) + b.st * ex2(db * ct);
-    r.s1 = a.s1 * ex2(da * LOG2E) + b.s1 * ex2(db * LOG2E);
-    return r;
+// the sums of `s` relative to the maximum m >= s.m
+template <bool BOTH>
+__device__ __forceinline__ void raise(Stats &s, float m, float ct) {
+    s.st *= ex2(scaled_max(s.m, ct) - scaled_max(m, ct));
+    if (BOTH) s.s1 *= ex2(scaled_max(s.m, LOG2E) - scaled_max(m, LOG2E));
+    s.m = m;
 }
 
 struct DistillArgs {
@@ -68,17 +67,15 @@ struct DistillArgs {
 };
 
 // Cluster of 1 to 8 blocks per row, a stretch of it each. BOTH: the hard part's
-// softmax (temperature 1) is needed beside the list's. CACHE: the stretch stays
-// in shared memory for the gradient; without it, it is read again.
-template <bool GRAD, bool BOTH, bool CACHE>
+// softmax (temperature 1) is needed beside the list's. Warp 0 looks after the
+// list; every thread reads from shared memory only what it copied there itself.
+template <bool GRAD, bool BOTH>
 __global__ void __launch_bounds__(NT)
 distill_kernel(DistillArgs a) {
-    extern __shared__ float4 slice4[];  // [cached stretch + 8], then the list: sp, sx, si [k]
+    extern __shared__ float4 slice4[];  // [stretch + 8], then the list: sp, sx, si [k]
     __shared__ Stats sw[NT / 32], sc[MAX_PARTS];
-    __shared__ float red[NT / 32];
-    __shared__ int twice;
-    float *slice = (float *)slice4;
-    float *sp = slice + (CACHE ? a.stretch + 8 : 0), *sx = sp + a.k;
+    __shared__ int twice, listed;
+    float *slice = (float *)slice4, *sp = slice + a.stretch + 8, *sx = sp + a.k;
     int *si = (int *)(sx + a.k);
     auto cluster = coop::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
@@ -91,205 +88,174 @@ distill_kernel(DistillArgs a) {
     // elements before the first 16-byte boundary, whole groups of four, the rest;
     // element i of the stretch is kept at slice[pad + i], groups at float4s
     const int head = min(n, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (n - head) / 4, pad = (4 - head) & 3;
-    const float4 *x4 = (const float4 *)(x + head);
+    const int odd = tid < head ? tid : tid < n - 4 * quads ? tid + 4 * quads : -1;  // this thread's of those at both ends
     float4 *s4 = (float4 *)(slice + pad + head);
+    for (int q = tid; q < quads; q += NT)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s4 + q)), "l"(x + head + 4 * q) : "memory");
+    if (odd >= 0)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slice + pad + odd)), "l"(x + odd) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
 
-    Stats s{-INFINITY, 0.0f, 0.0f};
-    auto add = [&](float v, float ref) {
-        const float d = v - ref;
-        s.st += ex2(d * ct);
-        if (BOTH) s.s1 += ex2(d * LOG2E);
-    };
-    auto raise = [&](float m) {  // to a maximum over what comes next
-        if (m > s.m) {
-            const float d = s.m - m;
-            s.st *= ex2(d * ct);
-            if (BOTH) s.s1 *= ex2(d * LOG2E);
-            s.m = m;
-        }
-        return ref_of(s.m);
-    };
-    {
-        const int i = tid < head ? tid : tid < n - 4 * quads ? tid + 4 * quads : -1;  // the odd ones at both ends
-        if (i >= 0) {
-            const float v = x[i];
-            if (CACHE) slice[pad + i] = v;
-            add(v, raise(v));
-        }
-    }
-    for (int q0 = tid; q0 < quads; q0 += QUADS * NT) {
-        float4 v[QUADS];
-#pragma unroll
-        for (int j = 0; j < QUADS; ++j)
-            v[j] = q0 + j * NT < quads ? __ldcs(x4 + q0 + j * NT) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        float m = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < QUADS; ++j) {
-            m = fmaxf(m, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
-            if (CACHE && q0 + j * NT < quads) s4[q0 + j * NT] = v[j];
-        }
-        const float ref = raise(m);
-#pragma unroll
-        for (int j = 0; j < QUADS; ++j) {
-            add(v[j].x, ref);
-            add(v[j].y, ref);
-            add(v[j].z, ref);
-            add(v[j].w, ref);
-        }
-    }
-    // the list: its softmax sp and the student's logits sx there, in every block
+    // the list, where it counts, and the student's logits at its tokens
     float lm = -INFINITY;
-    for (int j = tid; j < k; j += NT) {
-        const int i = a.ti[row * k + j];
-        const float v = a.tv[row * k + j];
-        const bool ok = i >= 0 && i < a.V && v > -INFINITY;
-        si[j] = ok ? i : -1;
-        sp[j] = ok ? v : -INFINITY;
-        sx[j] = ok ? xr[i] : 0.0f;
-        lm = fmaxf(lm, sp[j]);
-    }
     const int tgt = a.targets ? a.targets[row] : -1;
     const bool has_tgt = tgt >= 0 && tgt < a.V;
     const float xt = has_tgt ? xr[tgt] : 0.0f;
+    if (warp == 0) {
+        for (int j = lane; j < k; j += 32) {
+            const int i = a.ti[row * k + j];
+            const float v = a.tv[row * k + j];
+            const bool ok = i >= 0 && i < a.V && v > -INFINITY;
+            si[j] = ok ? i : -1;
+            sp[j] = ok ? v : -INFINITY;
+            sx[j] = ok ? xr[i] : 0.0f;
+            lm = fmaxf(lm, sp[j]);
+        }
+        lm = warp_max(lm);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-    // the row's statistics: lanes, warps, blocks, each in a fixed order
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stats b{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.st, o),
-                      __shfl_xor_sync(0xffffffffu, s.s1, o)};
-        // the lower lane's value first, so that both lanes form the same sum
-        s = (lane & o) ? merge(b, s, ct) : merge(s, b, ct);
+    // statistics of the thread, the warp, the block and the row, in a fixed order
+    Stats s{-INFINITY, 0.0f, 0.0f};
+    for (int q = tid; q < quads; q += NT) {
+        const float4 v = s4[q];
+        s.m = fmaxf(s.m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
-    lm = warp_max(lm);
-    if (lane == 0) {
-        sw[warp] = s;
-        red[warp] = lm;
+    if (odd >= 0) s.m = fmaxf(s.m, slice[pad + odd]);
+    {
+        const float m = warp_max(s.m), rt = scaled_max(m, ct), r1 = scaled_max(m, LOG2E);
+        auto add = [&](float v) {
+            s.st += ex2(fmaf(v, ct, -rt));
+            if (BOTH) s.s1 += ex2(fmaf(v, LOG2E, -r1));
+        };
+#pragma unroll 2
+        for (int q = tid; q < quads; q += NT) {
+            const float4 v = s4[q];
+            add(v.x);
+            add(v.y);
+            add(v.z);
+            add(v.w);
+        }
+        if (odd >= 0) add(slice[pad + odd]);
+        s.m = m;
+        s.st = warp_sum(s.st);
+        if (BOTH) s.s1 = warp_sum(s.s1);
     }
+    if (lane == 0) sw[warp] = s;
     __syncthreads();
-    s = sw[0];
-    lm = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / 32; ++w) {
-        s = merge(s, sw[w], ct);
-        lm = fmaxf(lm, red[w]);
-    }
+    auto join = [&](const Stats *v, int count) {
+        float m = v[0].m;
+        for (int w = 1; w < count; ++w) m = fmaxf(m, v[w].m);
+        Stats r{m, 0.0f, 0.0f};
+        for (int w = 0; w < count; ++w) {
+            Stats u = v[w];
+            raise<BOTH>(u, m, ct);
+            r.st += u.st;
+            r.s1 += u.s1;
+        }
+        return r;
+    };
     if (parts > 1) {
+        if (warp == 0) s = join(sw, NT / 32);
         cluster.barrier_wait();
         if (tid < parts) *cluster.map_shared_rank(&sc[part], tid) = s;
         cluster.sync();  // also: every block has read what another one will overwrite
-        s = sc[0];
-        for (int p = 1; p < parts; ++p) s = merge(s, sc[p], ct);
+        s = join(sc, parts);
+    } else {
+        s = join(sw, NT / 32);
     }
-    const float ref = ref_of(s.m);
+    const float rt = scaled_max(s.m, ct), r1 = scaled_max(s.m, LOG2E);
     const bool live = !(s.m == -INFINITY && s.st == 0.0f);
-    const bool soft = live && lm > -INFINITY, hard = live && has_tgt;
-    auto sum = [&](float v) {
-        v = warp_sum(v);
-        __syncthreads();
-        if (lane == 0) red[warp] = v;
-        __syncthreads();
-        v = red[0];
-#pragma unroll
-        for (int w = 1; w < NT / 32; ++w) v += red[w];
-        return v;
-    };
-    if (soft) {
-        const float it = 1.0f / a.tau;
-        float lz = 0.0f;
-        for (int j = tid; j < k; j += NT) lz += sp[j] > -INFINITY ? expf((sp[j] - lm) * it) : 0.0f;
-        lz = sum(lz);
-        const float llz = logf(lz), lst = logf(s.st);
+    lm = __shfl_sync(0xffffffffu, lm, 0);
+    if (tid == 0) twice = live && lm > -INFINITY;  // hands "soft" to the block until it counts company
+    bool soft = live && lm > -INFINITY;            // so far right in warp 0 alone
+    const bool hard = live && has_tgt;
+    if (warp == 0) {
         float loss = 0.0f;
-        for (int j = tid; j < k; j += NT) {
-            const float z = (sp[j] - lm) * it;
-            const float p = sp[j] > -INFINITY ? expf(z) / lz : 0.0f;
-            if (p > 0.0f) loss += p * ((z - llz) - ((sx[j] - ref) * it - lst));
-            sp[j] = p;
+        if (soft) {
+            const float it = 1.0f / a.tau;
+            float lz = 0.0f;
+            for (int j = lane; j < k; j += 32) lz += sp[j] > -INFINITY ? expf((sp[j] - lm) * it) : 0.0f;
+            lz = warp_sum(lz);
+            const float llz = logf(lz), l2 = log2f(s.st);
+            for (int j = lane; j < k; j += 32) {
+                const float z = (sp[j] - lm) * it;
+                const float p = sp[j] > -INFINITY ? expf(z) / lz : 0.0f;
+                if (p > 0.0f) loss += p * ((z - llz) - LN2 * (fmaf(sx[j], ct, -rt) - l2));
+                sp[j] = p;
+            }
+            loss = warp_sum(loss) * (a.alpha * a.tau * a.tau);
         }
-        if (part == 0) {
-            loss = sum(loss) * (a.alpha * a.tau * a.tau);
-            if (hard) loss += (1.0f - a.alpha) * (logf(s.s1) - (xt - ref));
-            if (tid == 0) a.row_loss[row] = loss;
-        }
-    } else if (part == 0 && tid == 0) {
-        a.row_loss[row] = hard ? (1.0f - a.alpha) * (logf(s.s1) - (xt - ref)) : 0.0f;
+        if (hard) loss -= (1.0f - a.alpha) * (LN2 * (fmaf(xt, LOG2E, -r1) - log2f(BOTH ? s.s1 : 1.0f)));
+        if (part == 0 && lane == 0) a.row_loss[row] = loss;
     }
     if (!GRAD) return;
+    __syncthreads();
+    soft = twice;
 
     float *dr = a.dlogits + row * a.ldd, *d = dr + lo;
-    const float gt = soft ? a.scale * a.alpha * a.tau / s.st : 0.0f;
-    const float g1 = BOTH && hard ? a.scale * (1.0f - a.alpha) / s.s1 : 0.0f;
     const float ot = a.scale * a.alpha * a.tau, o1 = a.scale * (1.0f - a.alpha);
+    const float gt = soft ? ot / s.st : 0.0f, g1 = BOTH && hard ? o1 / s.s1 : 0.0f;
+    const bool none = !soft && !hard;
     auto grad = [&](float v) {
-        const float e = v - ref;
-        // a part that is switched off counts as 0 whatever its exponential
-        float g = soft ? gt * ex2(e * ct) : 0.0f;
-        if (BOTH && hard) g = fmaf(g1, ex2(e * LOG2E), g);
-        return g;
+        float g = gt * ex2(fmaf(v, ct, -rt));
+        if (BOTH) g = fmaf(g1, ex2(fmaf(v, LOG2E, -r1)), g);
+        return none ? 0.0f : g;
     };
-    {
-        const int i = tid < head ? tid : tid < n - 4 * quads ? tid + 4 * quads : -1;
-        if (i >= 0) d[i] = grad(CACHE ? slice[pad + i] : x[i]);
-    }
-    const bool whole = ((uintptr_t)(d + head) & 15) == 0;  // the groups of x are groups of d too
-    for (int q = tid; q < quads; q += NT) {
-        float4 v = CACHE ? s4[q] : __ldcs(x4 + q);
-        v = make_float4(grad(v.x), grad(v.y), grad(v.z), grad(v.w));
-        if (whole) {
-            __stcs((float4 *)(d + head) + q, v);
-        } else {
-            float *p = d + head + 4 * q;
-            p[0] = v.x;
-            p[1] = v.y;
-            p[2] = v.z;
-            p[3] = v.w;
+    if (odd >= 0) d[odd] = grad(slice[pad + odd]);
+    if (((uintptr_t)(d + head) & 15) == 0) {  // the groups of x are groups of d too
+#pragma unroll 2
+        for (int q = tid; q < quads; q += NT) {
+            const float4 v = s4[q];
+            __stcs((float4 *)(d + head) + q, make_float4(grad(v.x), grad(v.y), grad(v.z), grad(v.w)));
         }
+    } else {  // another alignment: element by element, from the whole block's copies
+        for (int i = head + tid; i < head + 4 * quads; i += NT) d[i] = grad(slice[pad + i]);
     }
-    if (!soft && !hard) return;
+    if (none) return;
+    __syncthreads();
     // entries of the list and the target in this stretch: written again with
     // their own part taken off, by the first entry of a token for all of its
-    if (tid == 0) twice = !CACHE;
-    __syncthreads();
-    if (soft && CACHE) {
-        // the cached stretch has done its service: every entry leaves its number
-        // at its token, and one that finds another there has company
-        for (int j = tid; j < k; j += NT)
-            if (si[j] >= lo && si[j] < hi) slice[pad + si[j] - lo] = __int_as_float(j);
-        __syncthreads();
-        for (int j = tid; j < k; j += NT)
-            if (si[j] >= lo && si[j] < hi && __float_as_int(slice[pad + si[j] - lo]) != j) twice = 1;
-        __syncthreads();
+    if (warp != 0) return;
+    if (lane == 0) {
+        twice = 0;
+        listed = 0;
     }
-    const bool search = twice;
-    if (soft)
-        for (int j = tid; j < k; j += NT) {
-            const int i = si[j];
-            if (i < lo || i >= hi) continue;
+    __syncwarp();
+    auto mine = [&](int j) { return si[j] >= lo && si[j] < hi; };
+    if (soft) {
+        // the stretch has done its service: every entry leaves its number at its
+        // token, and one that finds another there has company
+        for (int j = lane; j < k; j += 32)
+            if (mine(j)) slice[pad + si[j] - lo] = __int_as_float(j);
+        __syncwarp();
+        for (int j = lane; j < k; j += 32)
+            if (mine(j)) {
+                if (__float_as_int(slice[pad + si[j] - lo]) != j) twice = 1;
+                if (si[j] == tgt) listed = 1;
+            }
+        __syncwarp();
+        const bool search = twice;
+        for (int j = lane; j < k; j += 32) {
+            if (!mine(j)) continue;
             float p = sp[j];
             if (search) {
                 bool first = true;
                 p = 0.0f;
                 for (int l = 0; l < k; ++l)
-                    if (si[l] == i) {
+                    if (si[l] == si[j]) {
                         first &= l >= j;
                         p += sp[l];
                     }
                 if (!first) continue;
             }
             float g = grad(sx[j]) - ot * p;
-            if (hard && i == tgt) g -= o1;
-            dr[i] = g;
+            if (hard && si[j] == tgt) g -= o1;
+            dr[si[j]] = g;
         }
-    if (hard && tgt >= lo && tgt < hi) {
-        __shared__ int listed;
-        if (tid == 0) listed = 0;
-        __syncthreads();
-        if (soft)
-            for (int j = tid; j < k; j += NT)
-                if (si[j] == tgt) listed = 1;
-        __syncthreads();
-        if (tid == 0 && !listed) dr[tgt] = grad(xt) - o1;
+        __syncwarp();
     }
+    if (hard && tgt >= lo && tgt < hi && lane == 0 && !listed) dr[tgt] = grad(xt) - o1;
 }
 
 // 1024 threads each sum a fixed strided subset, then a fixed-shape tree.
@@ -307,12 +273,12 @@ loss_sum_kernel(const float *__restrict__ row_loss, int rows, float scale, float
     if (threadIdx.x == 0) *loss = scale * sh[0];
 }
 
-template <bool GRAD, bool BOTH, bool CACHE>
+template <bool GRAD, bool BOTH>
 int launch(const DistillArgs &a, int rows, int parts, size_t smem, cudaStream_t s) {
     static bool set = false;
     if (!set) {
-        CG_CUDA(cudaFuncSetAttribute(distill_kernel<GRAD, BOTH, CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     SLICE_MAX + 12 * TOPK_MAX));
+        CG_CUDA(cudaFuncSetAttribute(distill_kernel<GRAD, BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     DISTILL_MAX_VOCAB / MAX_PARTS * 4 + 64 + 12 * TOPK_MAX));
         set = true;
     }
     cudaLaunchConfig_t cfg = {};
@@ -326,7 +292,7 @@ int launch(const DistillArgs &a, int rows, int parts, size_t smem, cudaStream_t 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    CG_CUDA(cudaLaunchKernelEx(&cfg, distill_kernel<GRAD, BOTH, CACHE>, a));
+    CG_CUDA(cudaLaunchKernelEx(&cfg, distill_kernel<GRAD, BOTH>, a));
     ++g_launch_count;
     return OK;
 }
@@ -350,14 +316,10 @@ int distill_rows(const float *logits, long ldl, int rows, int V, const float *tv
     }
     DistillArgs a{logits, ldl, V, ((V + parts - 1) / parts + 3) / 4 * 4, tv, ti, k, targets, tau, alpha, scale, row_loss,
                   dlogits, ldd};
-    const size_t list = (size_t)k * 12, bytes = ((size_t)a.stretch + 8) * sizeof(float);
-    const bool both = alpha < 1.0f && targets;
-    if (!dlogits)
-        return both ? launch<false, true, false>(a, rows, parts, list, s) : launch<false, false, false>(a, rows, parts, list, s);
-    if (bytes <= SLICE_MAX)
-        return both ? launch<true, true, true>(a, rows, parts, bytes + list, s)
-                    : launch<true, false, true>(a, rows, parts, bytes + list, s);
-    return both ? launch<true, true, false>(a, rows, parts, list, s) : launch<true, false, false>(a, rows, parts, list, s);
+    const size_t smem = ((size_t)a.stretch + 8) * sizeof(float) + (size_t)k * 12;
+    if (alpha < 1.0f && targets)
+        return dlogits ? launch<true, true>(a, rows, parts, smem, s) : launch<false, true>(a, rows, parts, smem, s);
+    return dlogits ? launch<true, false>(a, rows, parts, smem, s) : launch<false, false>(a, rows, parts, smem, s);
 }
 
 int distill_loss_sum(const float *row_loss, int rows, float scale, float *loss, cudaStream_t s) {

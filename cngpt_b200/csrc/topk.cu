@@ -145,7 +145,7 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
 #pragma unroll
         for (int j = 0; j < QUADS; ++j) {
             const int q = (c * QUADS + j) * NT + tid;
-            dst[j] = q < quads ? __ldcs(x4 + q) : make_float4(0.f, 0.f, 0.f, 0.f);
+            dst[j] = q < quads ? __ldcs(x4 + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         }
     };
     fetch(nx, 0);
@@ -153,24 +153,29 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
     if (tid < head) buf[atomicAdd(&sm.count, 1)] = make_key(x[tid], lo + tid);
     __syncthreads();
     const int chunks = (quads + QUADS * NT - 1) / (QUADS * NT);
-    bool all = true;     // fewer than k seen: every element is a candidate
-    float low = 0.0f;    // else those above low (any number if low is NaN)
-    bool any_number = false;
+    const int trigger = max(2 * k, TRIGGER);
+    bool all = true;  // fewer than k kept: every element is a candidate, NaN too
+    float low = 0.0f;
     for (int c = 0; c < chunks; ++c) {
 #pragma unroll
         for (int j = 0; j < QUADS; ++j) v[j] = nx[j];
         if (c + 1 < chunks) fetch(nx, c + 1);
         uint32_t pass = 0;
+        if (all) {
 #pragma unroll
-        for (int j = 0; j < QUADS; ++j) {
-            const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-            const bool in = (c * QUADS + j) * NT + tid < quads;
+            for (int j = 0; j < QUADS; ++j) pass |= (c * QUADS + j) * NT + tid < quads ? 0xFu << (4 * j) : 0u;
+        } else {
+            float mx = -INFINITY;  // what lies behind the row was read as -inf
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const bool p = all || (any_number ? e[y] == e[y] : e[y] > low);
-                pass |= (in && p) ? 1u << (4 * j + y) : 0u;
+            for (int j = 0; j < QUADS; ++j) mx = fmaxf(mx, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+            if (mx > low) {
+#pragma unroll
+                for (int j = 0; j < QUADS; ++j)
+                    pass |= ((v[j].x > low ? 1u : 0u) | (v[j].y > low ? 2u : 0u) | (v[j].z > low ? 4u : 0u) |
+                             (v[j].w > low ? 8u : 0u)) << (4 * j);
             }
         }
+        bool full = false;
         if (__any_sync(0xffffffffu, pass != 0)) {
             const int mine = __popc(pass);
             int inc = mine;
@@ -180,32 +185,30 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
                 if (lane >= o) inc += u;
             }
             int base = 0;
-            if (lane == 31) base = atomicAdd(&sm.count, inc);
+            if (lane == 31) {
+                base = atomicAdd(&sm.count, inc);
+                full = base + inc >= (all ? k + 1 : trigger);  // the last of the chunk to add sees the whole count
+            }
             int at = __shfl_sync(0xffffffffu, base, 31) + inc - mine;
-#pragma unroll
-            for (int j = 0; j < QUADS; ++j) {
-                const float e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-                    if (pass >> (4 * j + y) & 1)
-                        buf[at++] = make_key(e[y], (uint32_t)(lo + head + 4 * ((c * QUADS + j) * NT + tid) + y));
+            while (pass) {
+                const int b = __ffs(pass) - 1;
+                pass &= pass - 1;
+                const float4 f = b & 8 ? (b & 4 ? v[3] : v[2]) : (b & 4 ? v[1] : v[0]);
+                const float e = b & 2 ? (b & 1 ? f.w : f.z) : (b & 1 ? f.y : f.x);
+                buf[at++] = make_key(e, (uint32_t)(lo + head + 4 * ((c * QUADS + (b >> 2)) * NT + tid) + (b & 3)));
             }
         }
-        __syncthreads();
-        const int have = sm.count;
         // the buffer holds what may stay uncut and one more chunk
-        if (have > k && (all || have >= max(2 * k, TRIGGER))) {
-            select_k(buf, have, k, sm);
-            all = false;
+        if (__syncthreads_or(full)) {
+            select_k(buf, sm.count, k, sm);
+            // a worst one that is NaN lets every number pass; +-0 keeps its sign out of the comparison
+            all = sm.low == 0u;
             low = rank_value(sm.low);
-            any_number = sm.low == 0u;
-        } else {
-            __syncthreads();  // count has been read by all
         }
     }
     {  // the last ones (their indices are the highest, so they come last)
         const int i = head + 4 * quads + tid;
-        if (i < n && (all || (any_number ? x[i] == x[i] : x[i] > low))) buf[atomicAdd(&sm.count, 1)] = make_key(x[i], lo + i);
+        if (i < n && (all || x[i] > low)) buf[atomicAdd(&sm.count, 1)] = make_key(x[i], lo + i);
         __syncthreads();
     }
     const int seen = sm.count;

@@ -157,12 +157,12 @@ int cngpt_cuda_topk(const float *logits, long ld, int rows, int vocab, int k, fl
  * target lies outside [0, vocab) no hard part, a row with neither has loss 0
  * and gradient 0, and so has a row whose logits are all -inf. A vocabulary entry
  * of -inf has probability 0 (a teacher's token or a target there makes the loss
- * +inf, its gradient stays finite); NaN logits give NaN.
+ * +inf, its gradient stays finite); NaN and +inf logits give NaN.
  * targets may be NULL when alpha == 1, top_val and top_idx when alpha == 0 or
  * k == 0. dlogits NULL computes the loss alone; dlogits may be logits itself
  * (with ldd == ld), else the two must not overlap. Columns from vocab to ldd
  * are left as they are. loss: one float, row_loss: rows floats, both written.
- * temperature > 0, 0 <= alpha <= 1, 0 <= k <= 1024. All pointers are device
+ * temperature > 0, 0 <= alpha <= 1, 0 <= k <= 1024, vocab <= 400000. All pointers are device
  * pointers. The result does not depend on the order in which blocks run. */
 int cngpt_cuda_distill(const float *logits, long ld, int rows, int vocab, const float *top_val,
                        const int *top_idx, int k, const int *targets, float temperature, float alpha,
