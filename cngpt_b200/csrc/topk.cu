@@ -26,12 +26,21 @@ namespace coop = cooperative_groups;
 typedef unsigned long long u64;
 
 constexpr int NT = 256;              // threads
-constexpr int QUADS = 4;             // 16-byte loads of a thread and chunk
+#ifndef TK_Q
+#define TK_Q 4
+#define TK_OCC 4
+#endif
+constexpr int QUADS = TK_Q;             // 16-byte loads of a thread and chunk
 constexpr int CHUNK = NT * QUADS * 4;
 constexpr int BINS = 2048;           // radix 2^11
 constexpr int TRIGGER = 256;         // candidates below which no selection is worth its time
 
 __device__ __forceinline__ u64 make_key(float x, uint32_t i) { return ((u64)rank_key(x) << 32) | (0xFFFFFFFFu - i); }
+
+__device__ __forceinline__ float4 pick(const float4 (&v)[QUADS], int j) {
+    if constexpr (QUADS == 4) return j & 2 ? (j & 1 ? v[3] : v[2]) : (j & 1 ? v[1] : v[0]);
+    else return j & 1 ? v[1] : v[0];
+}
 
 struct Smem {
     // hist is also where a selection collects the k it keeps (TOPK_MAX * 8 bytes)
@@ -124,7 +133,7 @@ __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
 
 // Cluster of 1 to 8 blocks per row, each with a stretch of it; block 0 then
 // joins the stretches' candidates from the others' shared memory.
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, TK_OCC)
 topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__restrict__ values,
             int *__restrict__ indices, int stretch) {
     extern __shared__ u64 buf[];  // [max(2 k, TRIGGER) + CHUNK + 8]
@@ -156,6 +165,34 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
     const int trigger = max(2 * k, TRIGGER);
     bool all = true;  // fewer than k kept: every element is a candidate, NaN too
     float low = 0.0f;
+    if (k <= NT && chunks > 1) {
+        // A first bar from the first chunk: each warp's ceil(k / warps)-th largest
+        // of its lanes' maxima, the lowest of them. At least k elements of the
+        // chunk reach it, so what lies below it cannot count, nor can an equal one
+        // of a later chunk. If it is -inf, NaN may count: no bar then.
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) mx = fmaxf(mx, fmaxf(fmaxf(nx[j].x, nx[j].y), fmaxf(nx[j].z, nx[j].w)));
+        uint32_t key = rank_key(mx);
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)  // the lanes' keys in falling order
+#pragma unroll
+            for (int d = size >> 1; d > 0; d >>= 1) {
+                const uint32_t o = __shfl_xor_sync(0xffffffffu, key, d);
+                const bool up = ((lane & size) == 0) == ((lane & d) == 0);  // this lane takes the larger
+                key = up ? max(key, o) : min(key, o);
+            }
+        key = __shfl_sync(0xffffffffu, key, (k + NT / 32 - 1) / (NT / 32) - 1);
+        if (lane == 0) sm.warp[tid / 32] = key;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) key = min(key, sm.warp[w]);
+        if (key > RANK_NEG_INF) {
+            all = false;
+            low = rank_value(key);
+        }
+    }
+    bool first = !all;  // elements of the first chunk that equal the bar count
     for (int c = 0; c < chunks; ++c) {
 #pragma unroll
         for (int j = 0; j < QUADS; ++j) v[j] = nx[j];
@@ -168,12 +205,14 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
             float mx = -INFINITY;  // what lies behind the row was read as -inf
 #pragma unroll
             for (int j = 0; j < QUADS; ++j) mx = fmaxf(mx, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
-            if (mx > low) {
+            if (mx > low || (first && mx == low)) {
+                auto over = [&](float e) { return e > low || (first && e == low); };
 #pragma unroll
                 for (int j = 0; j < QUADS; ++j)
-                    pass |= ((v[j].x > low ? 1u : 0u) | (v[j].y > low ? 2u : 0u) | (v[j].z > low ? 4u : 0u) |
-                             (v[j].w > low ? 8u : 0u)) << (4 * j);
+                    pass |= ((over(v[j].x) ? 1u : 0u) | (over(v[j].y) ? 2u : 0u) | (over(v[j].z) ? 4u : 0u) |
+                             (over(v[j].w) ? 8u : 0u)) << (4 * j);
             }
+            first = false;
         }
         bool full = false;
         if (__any_sync(0xffffffffu, pass != 0)) {
@@ -193,7 +232,7 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
             while (pass) {
                 const int b = __ffs(pass) - 1;
                 pass &= pass - 1;
-                const float4 f = b & 8 ? (b & 4 ? v[3] : v[2]) : (b & 4 ? v[1] : v[0]);
+                const float4 f = pick(v, b >> 2);
                 const float e = b & 2 ? (b & 1 ? f.w : f.z) : (b & 1 ? f.y : f.x);
                 buf[at++] = make_key(e, (uint32_t)(lo + head + 4 * ((c * QUADS + (b >> 2)) * NT + tid) + (b & 3)));
             }
