@@ -26,26 +26,21 @@ namespace coop = cooperative_groups;
 typedef unsigned long long u64;
 
 constexpr int NT = 256;              // threads
-#ifndef TK_Q
-#define TK_Q 4
-#define TK_OCC 4
-#endif
-constexpr int QUADS = TK_Q;             // 16-byte loads of a thread and chunk
+constexpr int QUADS = 4;             // 16-byte loads of a thread and chunk
 constexpr int CHUNK = NT * QUADS * 4;
+#ifndef TK_T
+#define TK_T 448
+#endif
 constexpr int BINS = 2048;           // radix 2^11
-constexpr int TRIGGER = 256;         // candidates below which no selection is worth its time
+constexpr int TRIGGER = TK_T;         // candidates below which no selection is worth its time
 
 __device__ __forceinline__ u64 make_key(float x, uint32_t i) { return ((u64)rank_key(x) << 32) | (0xFFFFFFFFu - i); }
-
-__device__ __forceinline__ float4 pick(const float4 (&v)[QUADS], int j) {
-    if constexpr (QUADS == 4) return j & 2 ? (j & 1 ? v[3] : v[2]) : (j & 1 ? v[1] : v[0]);
-    else return j & 1 ? v[1] : v[0];
-}
 
 struct Smem {
     // hist is also where a selection collects the k it keeps (TOPK_MAX * 8 bytes)
     union {
         uint32_t hist[BINS];
+        uint4 hist4[BINS / 4];
         u64 keep[TOPK_MAX];
     };
     uint32_t warp[NT / 32];
@@ -55,12 +50,83 @@ struct Smem {
     uint32_t low;          // rank_key of the worst one kept
 };
 
+// The same cut for up to SMALL candidates by warp 0 alone, while the others wait
+// at the barrier behind it: it bisects the logits' bits with the candidates in
+// registers and, among those that equal the k-th, the index's. The 3 x 200
+// instructions of one warp take the place of some 5000 of all warps.
+constexpr int SMALL = 512;
+
+__device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
+    constexpr int PER = SMALL / 32;
+    const int lane = threadIdx.x & 31;
+    uint32_t key[PER], top = 0, bottom = 0xFFFFFFFFu;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = lane + 32 * j;
+        key[j] = i < n ? (uint32_t)(buf[i] >> 32) : 0u;
+        top = max(top, key[j]);
+        if (i < n) bottom = min(bottom, key[j]);
+    }
+    uint32_t hi = __reduce_max_sync(0xffffffffu, top), lo = __reduce_min_sync(0xffffffffu, bottom);
+    // lo: the highest value that at least k candidates reach
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) c += key[j] >= mid;
+        if (__reduce_add_sync(0xffffffffu, c) >= k) lo = mid;
+        else hi = mid - 1;
+    }
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        above += key[j] > lo;
+        equal += key[j] == lo && lane + 32 * j < n;
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    // of the equal ones the k - above with the largest inverted index
+    uint32_t bar = 0;
+    if (above + equal > k) {
+        uint32_t a = 0, b = 0xFFFFFFFFu;
+        while (a < b) {
+            const uint32_t mid = a + (b - a) / 2 + 1;
+            int c = 0;
+            for (int j = 0; j < PER; ++j) c += key[j] == lo && lane + 32 * j < n && (uint32_t)buf[lane + 32 * j] >= mid;
+            if (__reduce_add_sync(0xffffffffu, c) >= k - above) a = mid;
+            else b = mid - 1;
+        }
+        bar = a;
+    }
+    // compaction in place: a round's survivors never pass the round's own places
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = lane + 32 * j;
+        const u64 c = i < n ? buf[i] : 0;
+        const bool keep = i < n && (key[j] > lo || (key[j] == lo && (uint32_t)c >= bar));
+        const uint32_t mask = __ballot_sync(0xffffffffu, keep);
+        if (keep) buf[at + __popc(mask & ((1u << lane) - 1))] = c;
+        at += __popc(mask);
+        __syncwarp();
+    }
+    if (lane == 0) {
+        sm.count = k;
+        sm.low = lo;
+    }
+}
+
 // Cuts the n > k candidates in buf to the k largest (any order) and sets low.
 // Radix from the top: 11, 11 and 10 bits of the logit, then of the index (only
 // where equal logits straddle the cut); ends as soon as the bin that holds the
 // k-th is needed whole. hist is zero before and after.
 __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (n <= SMALL) {
+        if (warp == 0) select_small(buf, n, k, sm);
+        __syncthreads();
+        return;
+    }
     u64 prefix = 0;
     int need = k, top = 64;
     while (true) {
@@ -72,13 +138,12 @@ __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
         __syncthreads();
         // thread t sums 8 bins from the top; exclusive scan over the threads
         const int hi = BINS - 8 * tid;
-        uint32_t c[8], s = 0;
+        const uint4 q1 = sm.hist4[hi / 4 - 1], q0 = sm.hist4[hi / 4 - 2];
+        sm.hist4[hi / 4 - 1] = sm.hist4[hi / 4 - 2] = make_uint4(0, 0, 0, 0);
+        const uint32_t c[8] = {q1.w, q1.z, q1.y, q1.x, q0.w, q0.z, q0.y, q0.x};
+        uint32_t s = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            c[j] = sm.hist[hi - 1 - j];
-            sm.hist[hi - 1 - j] = 0;
-            s += c[j];
-        }
+        for (int j = 0; j < 8; ++j) s += c[j];
         uint32_t inc = s;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -126,14 +191,14 @@ __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
     __syncthreads();
     for (int i = tid; i < k; i += NT) buf[i] = sm.keep[i];
     __syncthreads();
-    for (int i = tid; i < BINS; i += NT) sm.hist[i] = 0;
+    for (int i = tid; i < 2 * k; i += NT) sm.hist[i] = 0;  // where keep was
     if (tid == 0) sm.count = k;
     __syncthreads();
 }
 
 // Cluster of 1 to 8 blocks per row, each with a stretch of it; block 0 then
 // joins the stretches' candidates from the others' shared memory.
-__global__ void __launch_bounds__(NT, TK_OCC)
+__global__ void __launch_bounds__(NT, 4)
 topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__restrict__ values,
             int *__restrict__ indices, int stretch) {
     extern __shared__ u64 buf[];  // [max(2 k, TRIGGER) + CHUNK + 8]
@@ -144,17 +209,21 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
     const int tid = threadIdx.x, lane = tid & 31;
     const int lo = min(V, part * stretch), hi = min(V, lo + stretch), n = hi - lo;
     const float *x = logits + row * ldl + lo;
-    for (int i = tid; i < BINS; i += NT) sm.hist[i] = 0;
+    for (int i = tid; i < BINS / 4; i += NT) sm.hist4[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) sm.count = 0;
     // elements before the first 16-byte boundary, whole groups of four, the rest
     const int head = min(n, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (n - head) / 4;
     const float4 *x4 = (const float4 *)(x + head);
     float4 v[QUADS], nx[QUADS];
+    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     auto fetch = [&](float4 *dst, int c) {
+        const float4 *p = x4 + c * QUADS * NT + tid;
+        if ((c + 1) * QUADS * NT <= quads) {
 #pragma unroll
-        for (int j = 0; j < QUADS; ++j) {
-            const int q = (c * QUADS + j) * NT + tid;
-            dst[j] = q < quads ? __ldcs(x4 + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            for (int j = 0; j < QUADS; ++j) dst[j] = __ldcs(p + j * NT);
+        } else {
+#pragma unroll
+            for (int j = 0; j < QUADS; ++j) dst[j] = (c * QUADS + j) * NT + tid < quads ? __ldcs(p + j * NT) : none;
         }
     };
     fetch(nx, 0);
@@ -192,58 +261,45 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
             low = rank_value(key);
         }
     }
-    bool first = !all;  // elements of the first chunk that equal the bar count
-    for (int c = 0; c < chunks; ++c) {
-#pragma unroll
-        for (int j = 0; j < QUADS; ++j) v[j] = nx[j];
-        if (c + 1 < chunks) fetch(nx, c + 1);
-        uint32_t pass = 0;
-        if (all) {
-#pragma unroll
-            for (int j = 0; j < QUADS; ++j) pass |= (c * QUADS + j) * NT + tid < quads ? 0xFu << (4 * j) : 0u;
-        } else {
-            float mx = -INFINITY;  // what lies behind the row was read as -inf
-#pragma unroll
-            for (int j = 0; j < QUADS; ++j) mx = fmaxf(mx, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
-            if (mx > low || (first && mx == low)) {
-                auto over = [&](float e) { return e > low || (first && e == low); };
-#pragma unroll
-                for (int j = 0; j < QUADS; ++j)
-                    pass |= ((over(v[j].x) ? 1u : 0u) | (over(v[j].y) ? 2u : 0u) | (over(v[j].z) ? 4u : 0u) |
-                             (over(v[j].w) ? 8u : 0u)) << (4 * j);
-            }
-            first = false;
-        }
+    // takes what `accept`s of a chunk; cuts where more than that might not fit
+    auto take = [&](int c, bool any, auto accept) {
         bool full = false;
-        if (__any_sync(0xffffffffu, pass != 0)) {
-            const int mine = __popc(pass);
-            int inc = mine;
+        if (any) {
+            uint32_t pass = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += u;
-            }
-            int base = 0;
-            if (lane == 31) {
-                base = atomicAdd(&sm.count, inc);
-                full = base + inc >= (all ? k + 1 : trigger);  // the last of the chunk to add sees the whole count
-            }
-            int at = __shfl_sync(0xffffffffu, base, 31) + inc - mine;
-            while (pass) {
-                const int b = __ffs(pass) - 1;
-                pass &= pass - 1;
-                const float4 f = pick(v, b >> 2);
-                const float e = b & 2 ? (b & 1 ? f.w : f.z) : (b & 1 ? f.y : f.x);
-                buf[at++] = make_key(e, (uint32_t)(lo + head + 4 * ((c * QUADS + (b >> 2)) * NT + tid) + (b & 3)));
+            for (int j = 0; j < QUADS; ++j)
+                if ((c * QUADS + j) * NT + tid < quads)
+                    pass |= ((accept(v[j].x) ? 1u : 0u) | (accept(v[j].y) ? 2u : 0u) | (accept(v[j].z) ? 4u : 0u) |
+                             (accept(v[j].w) ? 8u : 0u)) << (4 * j);
+            if (pass) {
+                int at = atomicAdd(&sm.count, __popc(pass));
+                full = at + __popc(pass) >= (all ? k + 1 : trigger);  // the last of the chunk to add sees the whole count
+                do {
+                    const int b = __ffs(pass) - 1;
+                    pass &= pass - 1;
+                    const float4 f = b & 8 ? (b & 4 ? v[3] : v[2]) : (b & 4 ? v[1] : v[0]);
+                    const float e = b & 2 ? (b & 1 ? f.w : f.z) : (b & 1 ? f.y : f.x);
+                    buf[at++] = make_key(e, (uint32_t)(lo + head + 4 * ((c * QUADS + (b >> 2)) * NT + tid) + (b & 3)));
+                } while (pass);
             }
         }
         // the buffer holds what may stay uncut and one more chunk
         if (__syncthreads_or(full)) {
             select_k(buf, sm.count, k, sm);
-            // a worst one that is NaN lets every number pass; +-0 keeps its sign out of the comparison
-            all = sm.low == 0u;
+            all = sm.low == 0u;  // a worst one that is NaN lets every number pass
             low = rank_value(sm.low);
         }
+    };
+    for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) v[j] = nx[j];
+        if (c + 1 < chunks) fetch(nx, c + 1);
+        float mx = -INFINITY;  // what lies behind the row was read as -inf
+#pragma unroll
+        for (int j = 0; j < QUADS; ++j) mx = fmaxf(mx, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+        if (c == 0 && !all) take(c, __any_sync(0xffffffffu, mx >= low), [&](float e) { return e >= low; });
+        else if (all) take(c, true, [](float) { return true; });
+        else take(c, __any_sync(0xffffffffu, mx > low), [&](float e) { return e > low; });
     }
     {  // the last ones (their indices are the highest, so they come last)
         const int i = head + 4 * quads + tid;
