@@ -278,7 +278,7 @@ int launch(const DistillArgs &a, int rows, int parts, size_t smem, cudaStream_t 
     static bool set = false;
     if (!set) {
         CG_CUDA(cudaFuncSetAttribute(distill_kernel<GRAD, BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     DISTILL_MAX_VOCAB / MAX_PARTS * 4 + 64 + 12 * TOPK_MAX));
+                                     ROW_MAX_VOCAB / MAX_PARTS * 4 + 64 + 12 * TOPK_MAX));
         set = true;
     }
     cudaLaunchConfig_t cfg = {};

@@ -704,7 +704,7 @@ extern "C" int cngpt_cuda_teacher_topk(GPT *m, FastCtx *f, const int *tokens, in
     ModelCtx *c = model_ctx(m);
     if (!c) return ERR_STATE;
     const int C = m->cfg.n_embd, V = m->cfg.vocab_size, L = m->cfg.n_layer, H = m->cfg.n_head;
-    if (!f || !tokens || B <= 0 || T <= 0 || T > m->cfg.block_size || k < 1 || k > V || k > TOPK_MAX) {
+    if (!f || !tokens || B <= 0 || T <= 0 || T > m->cfg.block_size || k < 1 || k > V || k > TOPK_MAX || V > ROW_MAX_VOCAB) {
         set_last_error(ERR_ARG, "teacher_topk: bad shape B=%d T=%d (block %d) k=%d (at most min(vocab=%d, %d))", B, T,
                        m->cfg.block_size, k, V, TOPK_MAX);
         return ERR_ARG;

@@ -125,7 +125,7 @@ int attention_decode_at(const float *q, long ldq, const float *kcache, const flo
 // by the callers.
 constexpr int SAMPLE_MAX_VOCAB = 262144;
 constexpr int TOPK_MAX = 1024;
-constexpr int DISTILL_MAX_VOCAB = 400000;
+constexpr int ROW_MAX_VOCAB = 400000;
 struct SampleRows {
     const float *logits;
     long ldl;  // 0: every row draws from the same logits

@@ -985,8 +985,8 @@ extern "C" int cngpt_cuda_distill_step(GPT *m, const int *tokens, const int *tar
                                        float beta1, float beta2, float eps, float wd, float grad_clip, float *loss_out) {
     ModelCtx *c = model_ctx(m);
     if (!c) return ERR_STATE;
-    if (m->cfg.vocab_size > DISTILL_MAX_VOCAB) {
-        set_last_error(ERR_ARG, "distill_step: vocab %d > %d unsupported", m->cfg.vocab_size, DISTILL_MAX_VOCAB);
+    if (m->cfg.vocab_size > ROW_MAX_VOCAB) {
+        set_last_error(ERR_ARG, "distill_step: vocab %d > %d unsupported", m->cfg.vocab_size, ROW_MAX_VOCAB);
         return ERR_ARG;
     }
     if (!tokens || (alpha < 1.0f && !targets) || k < 0 || k > TOPK_MAX || !(temperature > 0.0f) || !std::isfinite(temperature) ||

@@ -53,6 +53,10 @@ int rows_shape(const char *fn, long ld, int rows, int vocab) {
         set_last_error(ERR_ARG, "%s: bad shape rows=%d vocab=%d ld=%ld", fn, rows, vocab, ld);
         return ERR_ARG;
     }
+    if (vocab > ROW_MAX_VOCAB) {
+        set_last_error(ERR_ARG, "%s: vocab %d > %d unsupported", fn, vocab, ROW_MAX_VOCAB);
+        return ERR_ARG;
+    }
     return OK;
 }
 
@@ -100,10 +104,6 @@ extern "C" int cngpt_cuda_distill(const float *logits, long ld, int rows, int vo
                                   float scale, float *loss, float *row_loss, float *dlogits, long ldd) {
     const char *fn = "distill";
     CG_TRY(rows_shape(fn, ld, rows, vocab));
-    if (vocab > DISTILL_MAX_VOCAB) {
-        set_last_error(ERR_ARG, "%s: vocab %d > %d unsupported", fn, vocab, DISTILL_MAX_VOCAB);
-        return ERR_ARG;
-    }
     if (k < 0 || k > TOPK_MAX) {
         set_last_error(ERR_ARG, "%s: k=%d outside [0, %d]", fn, k, TOPK_MAX);
         return ERR_ARG;

@@ -28,11 +28,8 @@ typedef unsigned long long u64;
 constexpr int NT = 256;              // threads
 constexpr int QUADS = 4;             // 16-byte loads of a thread and chunk
 constexpr int CHUNK = NT * QUADS * 4;
-#ifndef TK_T
-#define TK_T 448
-#endif
 constexpr int BINS = 2048;           // radix 2^11
-constexpr int TRIGGER = TK_T;         // candidates below which no selection is worth its time
+constexpr int TRIGGER = 448;         // candidates below which no selection is worth its time
 
 __device__ __forceinline__ u64 make_key(float x, uint32_t i) { return ((u64)rank_key(x) << 32) | (0xFFFFFFFFu - i); }
 
@@ -170,7 +167,7 @@ __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
         prefix = (prefix << bits) | (u64)sm.bin;
         need = sm.need;
         top = shift;
-        if (sm.equal == need) break;
+        if (sm.equal == need || top == 0) break;  // at the last bit the keys differ
     }
     const u64 cut = prefix << top;
     if (tid == 0) {

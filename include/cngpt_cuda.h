@@ -137,7 +137,7 @@ int cngpt_cuda_sample(const float *logits, long ld, int rows, int vocab, const f
 /* ---- the k largest logits of every row --------------------------------------
  * values [rows, k] falling, indices [rows, k]; equal values are ordered by index
  * (the lower first), NaN ranks below -inf, and -0 equals (and is returned as) 0.
- * 1 <= k <= min(vocab, 1024). Device pointers. */
+ * 1 <= k <= min(vocab, 1024), vocab <= 400000. Device pointers. */
 int cngpt_cuda_topk(const float *logits, long ld, int rows, int vocab, int k, float *values, int *indices);
 
 /* ---- distillation from a teacher's top logits ----------------------------------
