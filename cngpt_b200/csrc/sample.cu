@@ -1,6 +1,24 @@
 // sample.cu - one token per row of logits from given uniform numbers, with
 // temperature, top-k, top-p and min-p of every row (cngpt_cuda_sample).
+//
+// A token's rank is that of its 64-bit key (ordered bits of the logit, then the
+// inverted index), its weight exp((l - max) / T) in fixed point: 2^SH parts of the
+// largest weight, SH = 62 - log2(vocabulary), at least one part if it is not zero
+// in 64-bit floating point. Sums of such weights are exact whatever their order,
+// so atomics and any split of the row give the same token, and a border between
+// two tokens is off by at most V / 2^(SH + 1) parts, 1e-9 of the largest weight.
+//
+// A cluster of blocks holds the row in shared memory. Both cuts of the ranking
+// (top-k: the first k keys; top-p: the keys before which less than p of the weight
+// lies) are thresholds on the key, found alike: a histogram of the counts or
+// weights over 1024 bins of max - l, whose prefix sums give the bin that the
+// border falls into; the few hundred keys of that bin are then compared with one
+// another. Where a bin holds more than that (runs of equal logits, outliers that
+// stretch the bins), it is cut again by the bits of its keys until it does not.
+#include <algorithm>
 #include <cmath>
+
+#include <cooperative_groups.h>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -9,191 +27,438 @@
 namespace cg {
 namespace {
 
-#define LAUNCH_CHECK() do { ++g_launch_count; CG_CUDA(cudaGetLastError()); } while (0)
+namespace coop = cooperative_groups;
 
-constexpr int NT = 1024;
+typedef unsigned long long u64;
 
-// Sum over the block in a fixed order, the same value in every thread.
-template <class T>
-__device__ T block_sum(T v, T *sh) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    T s = 0;
-    for (int w = 0; w < NT / 32; ++w) s += sh[w];
-    return s;
-}
+constexpr int NT = 256;
+constexpr int WARPS = NT / 32;
+constexpr int MAX_PARTS = 8;
+#ifndef SM_SLICE
+#define SM_SLICE 52
+#endif
+constexpr int SLICE_BYTES = SM_SLICE * 1024;  // of a row in a block's shared memory
+constexpr int BINS = 4 * NT;
+constexpr int BORDER = 512;  // keys that are compared with one another
+
+__device__ __forceinline__ u64 make_key(uint32_t rank, int i) { return ((u64)rank << 32) | (0xFFFFFFFFu - (uint32_t)i); }
+
+struct Border {  // what a block has of the border's bin
+    int count;
+    u64 lowest, highest;
+};
+
+struct Smem {
+    union {
+        struct {
+            uint32_t lo[BINS], hi[BINS];  // a bin's count, or its weight in two halves
+        };
+        struct {
+            u64 key[BORDER], measure[BORDER];  // the border's keys of all blocks
+        };
+    };
+    u64 list[BORDER];  // this block's keys of the border
+    Border mine;
+    float max_of[MAX_PARTS], min_of[MAX_PARTS];
+    u64 sum_of[MAX_PARTS];
+    int first_of[MAX_PARTS];
+    u64 warp[WARPS];
+    float fwarp[2][WARPS];
+    int bin;
+    u64 above, cut;
+};
 
 struct Row {
-    const float *x;
-    int V;
+    const float *s;  // the block's stretch in shared memory
+    int n, lo, per;  // its length, the index of its first token, tokens of a thread (odd: no bank conflicts)
     float mx;
-    double t;
-    uint32_t key;  // tokens with a higher key stay, and at this key those up to index `cut`
-    int cut;
-    __device__ bool keeps(int i, uint32_t k) const { return k > key || (k == key && i <= cut); }
-    __device__ double weight(int i) const {
-        const float l = x[i];
-        if (isinf(mx)) return l == mx ? 1.0 : 0.0;
-        return exp(((double)l - (double)mx) / t);
+    double m, it;    // maximum, 1 / temperature
+    int sh;
+    double tiny;     // exponents of less than half a part
+    u64 cut;         // keys below are out
+    __device__ float gap(float x) const { return x == mx ? 0.0f : mx - x; }
+    __device__ bool keeps(u64 key) const { return key >= cut; }
+    // exponent of the weight; -inf for a finite logit beside a maximum of +inf
+    __device__ double exponent(float x) const {
+        if (x == mx) return 0.0;
+        const double d = (double)x - m;
+        return isinf(d) ? d : d * it;
+    }
+    __device__ u64 weight(float x) const {
+        const double y = exponent(x);
+        if (y < tiny) return y < -745.0 ? 0 : 1;
+        return max(1ull, (u64)__double2ll_rn(ldexp(exp(y), sh)));
     }
 };
 
-// The threshold that keeps the kept tokens above `key`, and the first `m` (in
-// index order) at it.
-__device__ int nth_at_key(const Row &r, uint32_t key, int m, int *shi) {
-    int lo = 0, hi = r.V - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        int c = 0;
-        for (int i = threadIdx.x; i <= mid; i += NT) {
-            const uint32_t k = rank_key(r.x[i]);
-            c += k == key && r.keeps(i, k);
-        }
-        if (block_sum(c, shi) >= m) hi = mid;
-        else lo = mid + 1;
+// inclusive sum over the lanes up to this one
+__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
     }
-    return lo;
+    return v;
+}
+
+// Raises r.cut to the border of the ranking at which the measure of the tokens
+// before (their number, or WEIGHT) reaches a limit: `k`, or the part `p` of the
+// whole weight. The first token always stays.
+template <bool WEIGHT>
+__device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
+    auto cluster = coop::this_cluster();
+    const int parts = (int)cluster.num_blocks(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int i0 = min(r.n, tid * r.per), i1 = min(r.n, i0 + r.per);
+    u64 above = 0, limit = k, lowest = 0, highest = 0;
+    int shift = 0;
+    for (int level = 0;; ++level) {
+        // bin of a token, the best ones first; -1: not (any more) in question
+        auto bin_of = [&](float x, u64 key) {
+            if (level == 0) return r.keeps(key) ? (int)fminf(r.gap(x) * scale, (float)(BINS - 1)) : -1;
+            return key >= lowest && key <= highest ? (int)((highest - key) >> shift) : -1;
+        };
+        for (int b = tid; b < BINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
+        __syncthreads();
+        for (int i = i0; i < i1; ++i) {
+            const float x = r.s[i];
+            const int b = bin_of(x, make_key(rank_key(x), r.lo + i));
+            if (b < 0) continue;
+            if (!WEIGHT) {
+                atomicAdd(&sm.lo[b], 1u);
+            } else {
+                const u64 w = r.weight(x);
+                const uint32_t l = (uint32_t)w, old = atomicAdd(&sm.lo[b], l);
+                const uint32_t h = (uint32_t)(w >> 32) + (old + l < old ? 1u : 0u);  // with the carry
+                if (h) atomicAdd(&sm.hi[b], h);
+            }
+        }
+        cluster.sync();
+        // thread t sums bins 4 t .. 4 t + 3 over the blocks; exclusive scan
+        u64 c[4] = {}, s = 0;
+        for (int q = 0; q < parts; ++q) {
+            const uint4 l = *((const uint4 *)cluster.map_shared_rank(sm.lo, q) + tid);
+            c[0] += l.x;
+            c[1] += l.y;
+            c[2] += l.z;
+            c[3] += l.w;
+            if (WEIGHT) {
+                const uint4 h = *((const uint4 *)cluster.map_shared_rank(sm.hi, q) + tid);
+                c[0] += (u64)h.x << 32;
+                c[1] += (u64)h.y << 32;
+                c[2] += (u64)h.z << 32;
+                c[3] += (u64)h.w << 32;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += c[j];
+        const u64 inc = warp_scan(s, lane);
+        if (lane == 31) sm.warp[warp] = inc;
+        __syncthreads();
+        u64 before = above + inc - s, total = 0;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += sm.warp[w];
+            total += sm.warp[w];
+        }
+        if (level == 0) {
+            if (WEIGHT) limit = max(1ull, (u64)ceil(p * (double)total));
+            if (total <= limit) {  // nothing to cut (the same in every block)
+                cluster.sync();    // the bins have been read
+                return;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (before < limit && before + c[j] >= limit) {
+                sm.bin = 4 * tid + j;
+                sm.above = before;
+            }
+            before += c[j];
+        }
+        if (tid == 0) sm.mine = {0, ~0ull, 0};
+        __syncthreads();
+        above = sm.above;
+        const int bin = sm.bin;
+        u64 low = ~0ull, high = 0;
+        for (int i = i0; i < i1; ++i) {
+            const float x = r.s[i];
+            const u64 key = make_key(rank_key(x), r.lo + i);
+            if (bin_of(x, key) != bin) continue;
+            const int at = atomicAdd(&sm.mine.count, 1);
+            if (at < BORDER) sm.list[at] = key;
+            low = min(low, key);
+            high = max(high, key);
+        }
+        if (high) {
+            atomicMin(&sm.mine.lowest, low);
+            atomicMax(&sm.mine.highest, high);
+        }
+        cluster.sync();  // also: the bins have been read
+        int n = 0;
+        lowest = ~0ull;
+        highest = 0;
+        for (int q = 0; q < parts; ++q) {
+            const Border *b = cluster.map_shared_rank(&sm.mine, q);
+            n += b->count;
+            lowest = min(lowest, b->lowest);
+            highest = max(highest, b->highest);
+        }
+        if (n <= BORDER) {
+            int at = 0;
+            for (int q = 0; q < parts; ++q) {
+                const int m = cluster.map_shared_rank(&sm.mine, q)->count;
+                const u64 *other = cluster.map_shared_rank(sm.list, q);
+                for (int i = tid; i < m; i += NT) {
+                    const u64 key = other[i];
+                    sm.key[at + i] = key;
+                    if (WEIGHT) sm.measure[at + i] = r.weight(rank_value((uint32_t)(key >> 32)));
+                }
+                at += m;
+            }
+            if (tid == 0) sm.cut = ~0ull;
+            __syncthreads();
+            u64 cut = ~0ull;
+            for (int e = tid; e < n; e += NT) {
+                const u64 key = sm.key[e];
+                u64 b = above;
+                for (int j = 0; j < n; ++j)
+                    if (sm.key[j] > key) b += WEIGHT ? sm.measure[j] : 1;
+                if (b < limit) cut = min(cut, key);
+            }
+            if (cut != ~0ull) atomicMin(&sm.cut, cut);
+            __syncthreads();
+            r.cut = sm.cut;
+            return;
+        }
+        // 10 bits of the span of the keys that are left
+        shift = max(0, 64 - __clzll((long long)(highest - lowest)) - 10);
+    }
 }
 
 __global__ void __launch_bounds__(NT)
-sample_kernel(SampleRows a) {
-    __shared__ double shd[NT / 32];
-    __shared__ int shi[NT / 32];
-    __shared__ unsigned long long best;
-    __shared__ double part[NT];
-    const long row = blockIdx.x;
+sample_kernel(SampleRows a, int stretch, int sh) {
+    extern __shared__ float4 slice4[];
+    __shared__ __align__(16) Smem sm;
+    float *slice = (float *)slice4;
+    auto cluster = coop::this_cluster();
+    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    cluster.barrier_arrive();  // waited for before the first write to another block
+    const long row = blockIdx.x / parts, at = a.step ? (long)*a.step * a.rows + row : row;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Row r;
-    const int V = a.V;
-    const long at = a.step ? (long)*a.step * a.rows + row : row;
-    auto put = [&](int tok, float lp) {
-        a.tokens[at] = tok;
-        if (a.next) a.next[row] = max(tok, 0);
-        if (a.logprob) a.logprob[row] = lp;
+    r.lo = min(a.V, part * stretch);
+    r.n = min(a.V, r.lo + stretch) - r.lo;
+    r.per = ((r.n + NT - 1) / NT) | 1;
+    r.sh = sh;
+    r.tiny = -0.6931471805599453 * (sh + 1);
+    const float *x = a.logits + row * a.ldl + r.lo;
+    // elements before the first 16-byte boundary, whole groups of four, the rest;
+    // element i of the stretch is kept at slice[pad + i], groups at float4s
+    const int head = min(r.n, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (r.n - head) / 4, pad = (4 - head) & 3;
+    const int odd = tid < head ? tid : tid < r.n - 4 * quads ? tid + 4 * quads : -1;
+    float4 *s4 = (float4 *)(slice + pad + head);
+    for (int q = tid; q < quads; q += NT)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s4 + q)), "l"(x + head + 4 * q) : "memory");
+    if (odd >= 0)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slice + pad + odd)), "l"(x + odd) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const float T = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
+    const float min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[at];
+    const int k = a.top_k ? a.top_k[row] : 0;
+    auto put = [&](int token, float logprob) {
+        a.tokens[at] = token;
+        if (a.next) a.next[row] = max(token, 0);
+        if (a.logprob) a.logprob[row] = logprob;
     };
-    r.x = a.logits + row * a.ldl;
-    r.V = V;
-    const float T = a.temperature ? a.temperature[row] : 1.0f;
-    r.t = (double)T;
-    if (threadIdx.x == 0) best = 0;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    r.s = slice + pad;
+
+    // the row's largest logit and its smallest above -inf
+    float mx = -INFINITY, mn = INFINITY;
+    auto look = [&](float v) {
+        mx = fmaxf(mx, v);
+        mn = fminf(mn, v == -INFINITY ? INFINITY : v);
+    };
+    for (int q = tid; q < quads; q += NT) {
+        const float4 v = s4[q];
+        look(v.x);
+        look(v.y);
+        look(v.z);
+        look(v.w);
+    }
+    if (odd >= 0) look(r.s[odd]);
+    mx = warp_max(mx);
+    mn = -warp_max(-mn);
+    if (lane == 0) {
+        sm.fwarp[0][warp] = mx;
+        sm.fwarp[1][warp] = mn;
+    }
     __syncthreads();
-    unsigned long long b = 0;
-    for (int i = threadIdx.x; i < V; i += NT)
-        b = max(b, ((unsigned long long)rank_key(r.x[i]) << 32) | (0xFFFFFFFFu - (uint32_t)i));
-    atomicMax(&best, b);
-    __syncthreads();
-    const uint32_t bk = (uint32_t)(best >> 32);
-    const int bi = (int)(0xFFFFFFFFu - (uint32_t)best);
-    float p = a.top_p ? a.top_p[row] : 1.0f;
-    if (bk <= RANK_NEG_INF || !(T > 0.0f) || p <= 0.0f) {
-        if (threadIdx.x == 0) {
-            if (bk <= RANK_NEG_INF) put(-1, -INFINITY);
-            else put(bi, 0.0f);
+    for (int w = 0; w < WARPS; ++w) {
+        mx = fmaxf(mx, sm.fwarp[0][w]);
+        mn = fminf(mn, sm.fwarp[1][w]);
+    }
+    cluster.barrier_wait();
+    if (tid < parts) {
+        *cluster.map_shared_rank(&sm.max_of[part], tid) = mx;
+        *cluster.map_shared_rank(&sm.min_of[part], tid) = mn;
+    }
+    cluster.sync();
+    for (int q = 0; q < parts; ++q) {
+        mx = fmaxf(mx, sm.max_of[q]);
+        mn = fminf(mn, sm.min_of[q]);
+    }
+    if (mx == -INFINITY) {  // the same in every block, as all that follows
+        if (part == 0 && tid == 0) put(-1, -INFINITY);
+        return;
+    }
+    const int i0 = min(r.n, tid * r.per), i1 = min(r.n, i0 + r.per);
+    if (!(T > 0.0f) || p <= 0.0f) {  // the first of the ranking
+        int first = 0x7FFFFFFF;
+        for (int i = i0; i < i1; ++i)
+            if (r.s[i] == mx) {
+                first = r.lo + i;
+                break;
+            }
+        first = (int)__reduce_min_sync(0xffffffffu, (unsigned)first);
+        if (lane == 0) sm.warp[warp] = (u64)first;
+        __syncthreads();
+        for (int w = 0; w < WARPS; ++w) first = min(first, (int)sm.warp[w]);
+        if (tid == 0) *cluster.map_shared_rank(&sm.first_of[part], 0) = first;
+        cluster.sync();
+        if (part == 0 && tid == 0) {
+            for (int q = 0; q < parts; ++q) first = min(first, sm.first_of[q]);
+            put(first, 0.0f);
         }
         return;
     }
-    r.mx = rank_value(bk);
-    r.key = RANK_NEG_INF;
-    r.cut = -1;
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < V) {
-        // the lowest key that fewer than k keys exceed: the k-th largest
-        uint32_t lo = RANK_NEG_INF, hi = 0xFFFFFFFFu;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            int c = 0;
-            for (int i = threadIdx.x; i < V; i += NT) c += rank_key(r.x[i]) > mid;
-            if (block_sum(c, shi) < k) hi = mid;
-            else lo = mid + 1;
-        }
-        if (lo > RANK_NEG_INF) {
-            int c = 0;
-            for (int i = threadIdx.x; i < V; i += NT) c += rank_key(r.x[i]) > lo;
-            c = block_sum(c, shi);
-            r.key = lo - 1;  // all at `lo` while their order is looked at
-            const int cut = nth_at_key(r, lo, k - c, shi);
-            r.key = lo;
-            r.cut = cut;
-        }
-    }
-    auto mass = [&](uint32_t above) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < V; i += NT) {
-            const uint32_t kk = rank_key(r.x[i]);
-            if (kk > above && r.keeps(i, kk)) s += r.weight(i);
-        }
-        return block_sum(s, shd);
+    r.mx = mx;
+    r.m = (double)mx;
+    r.it = 1.0 / (double)T;
+    r.cut = (u64)(RANK_NEG_INF + 1) << 32;
+    // bins over the row's span, at most 64 wide (an outlier would stretch them)
+    const float scale = mn < mx ? fminf((float)BINS / fminf(mx - mn, 64.0f), 1e30f) : 0.0f;
+    if (k > 0 && k < a.V) cut_ranking<false>(r, scale, (u64)k, 0.0, sm);
+    if (p < 1.0f) cut_ranking<true>(r, scale, 0, (double)p, sm);
+    const double least = min_p > 0.0f ? log(fmin(1.0, (double)min_p)) : -INFINITY;
+
+    // cumulative weights in index order: threads, warps, blocks
+    auto drawn = [&](int i) -> u64 {
+        const float v = r.s[i];
+        if (!r.keeps(make_key(rank_key(v), r.lo + i)) || r.exponent(v) < least) return 0;
+        return r.weight(v);
     };
-    if (p < 1.0f) {
-        const double want = (double)p * mass(RANK_NEG_INF);
-        uint32_t lo = r.key, hi = 0xFFFFFFFFu;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (mass(mid) < want) hi = mid;
-            else lo = mid + 1;
-        }
-        if (lo > RANK_NEG_INF) {
-            const double above = mass(lo);
-            const double w = isinf(r.mx) ? 1.0 : exp(((double)rank_value(lo) - (double)r.mx) / r.t);
-            const double m = w > 0.0 ? ceil((want - above) / w) : (double)V;
-            if (m < (double)V) {
-                const int cut = nth_at_key(r, lo, max(1, (int)m), shi);
-                r.cut = r.key == lo ? min(r.cut, cut) : cut;
-                r.key = lo;
-            }
-        }
-    }
-    const float mp = a.min_p ? a.min_p[row] : 0.0f;
-    const double floor_w = mp > 0.0f ? (double)fminf(1.0f, mp) : 0.0;  // NaN: off
-    auto drawn = [&](int i) {
-        const uint32_t kk = rank_key(r.x[i]);
-        if (!r.keeps(i, kk)) return 0.0;
-        const double w = r.weight(i);
-        return w < floor_w ? 0.0 : w;
-    };
-    // index order: every thread sums its own stretch, the crossing stretch is walked
-    const int n = (V + NT - 1) / NT, i0 = min(V, (int)threadIdx.x * n), i1 = min(V, i0 + n);
-    double s = 0.0;
+    u64 s = 0;
     for (int i = i0; i < i1; ++i) s += drawn(i);
-    part[threadIdx.x] = s;
+    const u64 inc = warp_scan(s, lane);
+    if (lane == 31) sm.warp[warp] = inc;
     __syncthreads();
-    if (threadIdx.x != 0) return;
-    double total = 0.0;
-    for (int t = 0; t < NT; ++t) total += part[t];
-    const double target = (double)a.u[at] * total;
-    double c = 0.0;
-    int tok = bi;
-    double wt = 1.0;
-    for (int t = 0; t < NT; ++t) {
-        if (part[t] <= 0.0) continue;
-        const bool here = c + part[t] > target;
-        double c2 = c;
-        bool hit = false;
-        for (int i = t * n; i < min(V, t * n + n); ++i) {
-            const double w = drawn(i);
-            if (w <= 0.0) continue;
-            c2 += w;
-            tok = i;
-            wt = w;
-            if (here && c2 > target) {
-                hit = true;
-                break;
-            }
-        }
-        if (hit) break;
-        c += part[t];
+    u64 before = inc - s, block = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += sm.warp[w];
+        block += sm.warp[w];
     }
-    put(tok, (float)log(wt / total));
+    if (tid < parts) *cluster.map_shared_rank(&sm.sum_of[part], tid) = block;
+    cluster.sync();
+    u64 total = 0;
+    for (int q = 0; q < parts; ++q) {
+        if (q < part) before += sm.sum_of[q];
+        total += sm.sum_of[q];
+    }
+    // the first token whose cumulative weight exceeds u total: an integer that
+    // exceeds floor(u total)
+    const u64 target = u < 1.0f ? min(total - 1, (u64)fmax(0.0, (double)u * (double)total)) : total - 1;
+    if (target == 0 && u > 0.0f) {
+        // A number below one part of the whole: what the parts round up decides, so
+        // the weights are summed as they are. No generator of 24 or 32 bits gives
+        // such a number, so one thread walks the stretch that holds the border.
+        const double tau = ldexp((double)u * (double)total, -sh);
+        auto real = [&](int i) { return drawn(i) ? exp(r.exponent(r.s[i])) : 0.0; };
+        double d = 0.0;
+        for (int i = i0; i < i1; ++i) d += real(i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        __syncthreads();
+        if (lane == 0) sm.warp[warp] = (u64)__double_as_longlong(d);
+        __syncthreads();
+        d = 0.0;
+        for (int w = 0; w < WARPS; ++w) d += __longlong_as_double((long long)sm.warp[w]);
+        cluster.sync();  // sum_of has been read
+        if (tid < parts) *cluster.map_shared_rank(&sm.sum_of[part], tid) = (u64)__double_as_longlong(d);
+        cluster.sync();
+        double base = 0.0;
+        int owner = 0;
+        for (; owner < parts - 1; ++owner) {
+            const double next = base + __longlong_as_double((long long)sm.sum_of[owner]);
+            if (next > tau) break;
+            base = next;
+        }
+        if (part != owner || tid != 0) return;
+        int token = 0;
+        for (int i = 0; i < r.n; ++i) {
+            const double w = real(i);
+            if (w > 0.0) token = i;
+            base += w;
+            if (base > tau) break;
+        }
+        put(r.lo + token, (float)(r.exponent(r.s[token]) - log(ldexp((double)total, -sh))));
+        return;
+    }
+    const bool here = before <= target && before + s > target;
+    const uint32_t who = __ballot_sync(0xffffffffu, here);
+    if (!who) return;
+    const int owner = __ffs(who) - 1, o0 = __shfl_sync(0xffffffffu, i0, owner), o1 = __shfl_sync(0xffffffffu, i1, owner);
+    u64 c = __shfl_sync(0xffffffffu, before, owner);
+    for (int i = o0; i < o1; i += 32) {
+        const u64 w = i + lane < o1 ? drawn(i + lane) : 0;
+        const u64 sum = c + warp_scan(w, lane);
+        const uint32_t over = __ballot_sync(0xffffffffu, sum > target);
+        if (over) {
+            if (lane == __ffs(over) - 1) {
+                const float v = r.s[i + lane];
+                put(r.lo + i + lane, (float)(r.exponent(v) - log(ldexp((double)total, -sh))));
+            }
+            return;
+        }
+        c = __shfl_sync(0xffffffffu, sum, 31);
+    }
 }
 
 }  // namespace
 
 int sample_rows(const SampleRows &a, cudaStream_t s) {
     if (a.rows <= 0) return OK;
-    sample_kernel<<<a.rows, NT, 0, s>>>(a);
-    LAUNCH_CHECK();
+    // Blocks of a row: as many as the shared memory for its stretches asks for,
+    // more while there are rows for half the SMs at most.
+    int parts = 1;
+    while (parts < MAX_PARTS && ((long)a.V * 4 > (long)parts * SLICE_BYTES ||
+                                 ((long)a.rows * parts * 2 <= num_sms() && a.V >= parts * 2048)))
+        parts *= 2;
+    if ((long)a.rows * parts > 0x7FFFFFFFL) {
+        set_last_error(ERR_ARG, "sample: %d rows are too many", a.rows);
+        return ERR_ARG;
+    }
+    const int stretch = ((a.V + parts - 1) / parts + 3) / 4 * 4;
+    int sh = 62;
+    while (sh > 0 && (a.V - 1) >> (62 - sh)) --sh;  // V weights of 2^sh stay below 2^62
+    static bool set = false;
+    if (!set) {
+        CG_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (SAMPLE_MAX_VOCAB / MAX_PARTS + 16) * 4));
+        set = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.rows * parts));
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = ((size_t)stretch + 8) * sizeof(float);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CG_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel, a, stretch, sh));
+    ++g_launch_count;
     return OK;
 }
 
