@@ -3,7 +3,7 @@
 //
 // A token's rank is that of its 64-bit key (ordered bits of the logit, then the
 // inverted index), its weight exp((l - max) / T) in fixed point: 2^SH parts of the
-// largest weight, SH = 62 - log2(vocabulary), at least one part if it is not zero
+// largest weight, SH = 62 - log2(vocabulary), 50 at most, at least one part if it is not zero
 // in 64-bit floating point. Sums of such weights are exact whatever their order,
 // so atomics and any split of the row give the same token, and a border between
 // two tokens is off by at most V / 2^(SH + 1) parts, 1e-9 of the largest weight.
@@ -39,6 +39,7 @@ constexpr int MAX_PARTS = 8;
 #endif
 constexpr int SLICE_BYTES = SM_SLICE * 1024;  // of a row in a block's shared memory
 constexpr int BINS = 4 * NT;
+constexpr int TABLE = 64;    // entries 2^(j / 64) of the exponential
 constexpr int BORDER = 512;  // keys that are compared with one another
 
 __device__ __forceinline__ u64 make_key(uint32_t rank, int i) { return ((u64)rank << 32) | (0xFFFFFFFFu - (uint32_t)i); }
@@ -57,11 +58,15 @@ struct Smem {
             u64 key[BORDER], measure[BORDER];  // the border's keys of all blocks
         };
     };
+    double table[TABLE];
     u64 list[BORDER];  // this block's keys of the border
     Border mine;
     float max_of[MAX_PARTS], min_of[MAX_PARTS];
     u64 sum_of[MAX_PARTS];
     int first_of[MAX_PARTS];
+    uint32_t fine_lo[NT], fine_hi[NT];
+    short list_of[BORDER];
+    int few;
     u64 warp[WARPS];
     float fwarp[2][WARPS];
     int bin;
@@ -73,21 +78,40 @@ struct Row {
     int n, lo, per;  // its length, the index of its first token, tokens of a thread (odd: no bank conflicts)
     float mx;
     double m, it;    // maximum, 1 / temperature
+    double c;        // TABLE log2(e) / temperature
     int sh;
-    double tiny;     // exponents of less than half a part
-    u64 cut;         // keys below are out
+    const double *table;
+    float cut_at;    // tokens above this logit stay, and of those at it
+    int cut_index;   // the ones up to this index
+
+    __device__ bool keeps(float x, int i) const { return x > cut_at || (x == cut_at && i <= cut_index); }
     __device__ float gap(float x) const { return x == mx ? 0.0f : mx - x; }
-    __device__ bool keeps(u64 key) const { return key >= cut; }
-    // exponent of the weight; -inf for a finite logit beside a maximum of +inf
+    __device__ void cut(u64 key) {
+        cut_at = rank_value((uint32_t)(key >> 32));
+        cut_index = (int)(0xFFFFFFFFu - (uint32_t)key);
+    }
+    // log of the weight; -inf for a finite logit beside a maximum of +inf
     __device__ double exponent(float x) const {
         if (x == mx) return 0.0;
         const double d = (double)x - m;
         return isinf(d) ? d : d * it;
     }
+    // The weight in parts: 2^(z / 64) with z = k + f, |f| <= 1/2, as the table's
+    // 2^((k mod 64) / 64), its exponent raised by k / 64 + sh, times the Taylor
+    // series of 2^(f / 64) (the fifth power, 4e-14 of the weight, is left out).
+    // Adding 1.5 2^52 (2^52) leaves a rounded integer in the low bits.
     __device__ u64 weight(float x) const {
-        const double y = exponent(x);
-        if (y < tiny) return y < -745.0 ? 0 : 1;
-        return max(1ull, (u64)__double2ll_rn(ldexp(exp(y), sh)));
+        constexpr double B = 0.6931471805599453 / TABLE;
+        if (x == mx) return 1ull << sh;
+        const double z = ((double)x - m) * c;
+        if (z < -(double)(TABLE * (sh + 1))) return z < -745.0 / B ? 0 : 1;  // less than half a part
+        const double kd = z + 6755399441055744.0;
+        const int k = __double2loint(kd);
+        const double f = z - (kd - 6755399441055744.0);
+        const double q = fma(fma(fma(fma(B * B * B * B / 24, f, B * B * B / 6), f, B * B / 2), f, B), f, 1.0);
+        const double t = table[k & (TABLE - 1)];
+        const double w = __hiloint2double(__double2hiint(t) + ((k >> 6) + sh) * (1 << 20), __double2loint(t)) * q;
+        return max(1ull, (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull);
     }
 };
 
@@ -101,7 +125,7 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
     return v;
 }
 
-// Raises r.cut to the border of the ranking at which the measure of the tokens
+// Raises r's cut to the border of the ranking at which the measure of the tokens
 // before (their number, or WEIGHT) reaches a limit: `k`, or the part `p` of the
 // whole weight. The first token always stays.
 template <bool WEIGHT>
@@ -113,15 +137,17 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
     int shift = 0;
     for (int level = 0;; ++level) {
         // bin of a token, the best ones first; -1: not (any more) in question
-        auto bin_of = [&](float x, u64 key) {
-            if (level == 0) return r.keeps(key) ? (int)fminf(r.gap(x) * scale, (float)(BINS - 1)) : -1;
+        auto bin_of = [&](float x, int i) {
+            if (level == 0) return r.keeps(x, i) ? (int)fminf(r.gap(x) * scale, (float)(BINS - 1)) : -1;
+            const u64 key = make_key(rank_key(x), i);
             return key >= lowest && key <= highest ? (int)((highest - key) >> shift) : -1;
         };
-        for (int b = tid; b < BINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
+        *((uint4 *)sm.lo + tid) = make_uint4(0, 0, 0, 0);
+        *((uint4 *)sm.hi + tid) = make_uint4(0, 0, 0, 0);
         __syncthreads();
         for (int i = i0; i < i1; ++i) {
             const float x = r.s[i];
-            const int b = bin_of(x, make_key(rank_key(x), r.lo + i));
+            const int b = bin_of(x, r.lo + i);
             if (b < 0) continue;
             if (!WEIGHT) {
                 atomicAdd(&sm.lo[b], 1u);
@@ -181,8 +207,8 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
         u64 low = ~0ull, high = 0;
         for (int i = i0; i < i1; ++i) {
             const float x = r.s[i];
+            if (bin_of(x, r.lo + i) != bin) continue;
             const u64 key = make_key(rank_key(x), r.lo + i);
-            if (bin_of(x, key) != bin) continue;
             const int at = atomicAdd(&sm.mine.count, 1);
             if (at < BORDER) sm.list[at] = key;
             low = min(low, key);
@@ -193,40 +219,81 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
             atomicMax(&sm.mine.highest, high);
         }
         cluster.sync();  // also: the bins have been read
-        int n = 0;
+        // every warp: lane q asks block q, then warp q fetches block q's keys
+        int have = 0;
         lowest = ~0ull;
         highest = 0;
-        for (int q = 0; q < parts; ++q) {
-            const Border *b = cluster.map_shared_rank(&sm.mine, q);
-            n += b->count;
-            lowest = min(lowest, b->lowest);
-            highest = max(highest, b->highest);
+        if (lane < parts) {
+            const Border *b = cluster.map_shared_rank(&sm.mine, lane);
+            have = b->count;
+            lowest = b->lowest;
+            highest = b->highest;
         }
+        int upto = have;
+#pragma unroll
+        for (int o = 1; o < MAX_PARTS; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+            lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, o));
+            highest = max(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+        }
+        lowest = __shfl_sync(0xffffffffu, lowest, 0);
+        highest = __shfl_sync(0xffffffffu, highest, 0);
+        const int n = __shfl_sync(0xffffffffu, upto, MAX_PARTS - 1);
         if (n <= BORDER) {
-            int at = 0;
-            for (int q = 0; q < parts; ++q) {
-                const int m = cluster.map_shared_rank(&sm.mine, q)->count;
-                const u64 *other = cluster.map_shared_rank(sm.list, q);
-                for (int i = tid; i < m; i += NT) {
+            if (warp < parts) {
+                const int m = __shfl_sync(0xffffffffu, have, warp), at = __shfl_sync(0xffffffffu, upto, warp) - m;
+                const u64 *other = cluster.map_shared_rank(sm.list, warp);
+                for (int i = lane; i < m; i += 32) {
                     const u64 key = other[i];
                     sm.key[at + i] = key;
                     if (WEIGHT) sm.measure[at + i] = r.weight(rank_value((uint32_t)(key >> 32)));
                 }
-                at += m;
             }
-            if (tid == 0) sm.cut = ~0ull;
+            // the border among the keys: 256 bins of their span first, one a thread
+            const int fine = max(0, 64 - __clzll((long long)(highest - lowest)) - 8);
+            auto fine_of = [&](u64 key) { return (int)((highest - key) >> fine); };
+            sm.fine_lo[tid] = sm.fine_hi[tid] = 0;
+            if (tid == 0) {
+                sm.cut = ~0ull;
+                sm.few = 0;
+            }
             __syncthreads();
-            u64 cut = ~0ull;
             for (int e = tid; e < n; e += NT) {
-                const u64 key = sm.key[e];
-                u64 b = above;
-                for (int j = 0; j < n; ++j)
-                    if (sm.key[j] > key) b += WEIGHT ? sm.measure[j] : 1;
+                const int f = fine_of(sm.key[e]);
+                const u64 w = WEIGHT ? sm.measure[e] : 1;
+                const uint32_t l = (uint32_t)w, old = atomicAdd(&sm.fine_lo[f], l);
+                const uint32_t h = (uint32_t)(w >> 32) + (old + l < old ? 1u : 0u);
+                if (h) atomicAdd(&sm.fine_hi[f], h);
+            }
+            __syncthreads();
+            const u64 mine = ((u64)sm.fine_hi[tid] << 32) + sm.fine_lo[tid], scan = warp_scan(mine, lane);
+            if (lane == 31) sm.warp[warp] = scan;
+            __syncthreads();
+            u64 base = above + scan - mine;
+            for (int w = 0; w < warp; ++w) base += sm.warp[w];
+            if (base < limit && base + mine >= limit) {
+                sm.bin = tid;
+                sm.above = base;
+            }
+            __syncthreads();
+            for (int e = tid; e < n; e += NT)
+                if (fine_of(sm.key[e]) == sm.bin) sm.list_of[atomicAdd(&sm.few, 1)] = (short)e;
+            __syncthreads();
+            // each of those few against the others
+            u64 cut = ~0ull;
+            for (int e = tid; e < sm.few; e += NT) {
+                const u64 key = sm.key[sm.list_of[e]];
+                u64 b = sm.above;
+                for (int j = 0; j < sm.few; ++j) {
+                    const int o = sm.list_of[j];
+                    if (sm.key[o] > key) b += WEIGHT ? sm.measure[o] : 1;
+                }
                 if (b < limit) cut = min(cut, key);
             }
             if (cut != ~0ull) atomicMin(&sm.cut, cut);
             __syncthreads();
-            r.cut = sm.cut;
+            r.cut(sm.cut);
             return;
         }
         // 10 bits of the span of the keys that are left
@@ -249,7 +316,7 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     r.n = min(a.V, r.lo + stretch) - r.lo;
     r.per = ((r.n + NT - 1) / NT) | 1;
     r.sh = sh;
-    r.tiny = -0.6931471805599453 * (sh + 1);
+    r.table = sm.table;
     const float *x = a.logits + row * a.ldl + r.lo;
     // elements before the first 16-byte boundary, whole groups of four, the rest;
     // element i of the stretch is kept at slice[pad + i], groups at float4s
@@ -264,6 +331,7 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     const float T = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
     const float min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[at];
     const int k = a.top_k ? a.top_k[row] : 0;
+    if (tid < TABLE) sm.table[tid] = exp2((double)tid / TABLE);
     auto put = [&](int token, float logprob) {
         a.tokens[at] = token;
         if (a.next) a.next[row] = max(token, 0);
@@ -334,21 +402,31 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     r.mx = mx;
     r.m = (double)mx;
     r.it = 1.0 / (double)T;
-    r.cut = (u64)(RANK_NEG_INF + 1) << 32;
+    r.c = TABLE * 1.4426950408889634 * r.it;
+    r.cut_at = -INFINITY;
+    r.cut_index = -1;
     // bins over the row's span, at most 64 wide (an outlier would stretch them)
     const float scale = mn < mx ? fminf((float)BINS / fminf(mx - mn, 64.0f), 1e30f) : 0.0f;
     if (k > 0 && k < a.V) cut_ranking<false>(r, scale, (u64)k, 0.0, sm);
     if (p < 1.0f) cut_ranking<true>(r, scale, 0, (double)p, sm);
-    const double least = min_p > 0.0f ? log(fmin(1.0, (double)min_p)) : -INFINITY;
+    if (min_p > 0.0f) {
+        // log w >= log min_p as a bound on the logit, rounded up to the next one
+        const double least = log(fmin(1.0, (double)min_p));
+        const float bound = least < 0.0 ? __double2float_ru(r.m + least * (double)T) : mx;
+        if (bound > r.cut_at) r.cut(make_key(rank_key(bound), 0x7FFFFFFF));
+    }
 
     // cumulative weights in index order: threads, warps, blocks
     auto drawn = [&](int i) -> u64 {
         const float v = r.s[i];
-        if (!r.keeps(make_key(rank_key(v), r.lo + i)) || r.exponent(v) < least) return 0;
-        return r.weight(v);
+        return r.keeps(v, r.lo + i) ? r.weight(v) : 0;
     };
     u64 s = 0;
-    for (int i = i0; i < i1; ++i) s += drawn(i);
+    for (int j = i0; j < i1; j += 32) {  // which of 32 stay, then the weights of those alone
+        uint32_t stay = 0;
+        for (int i = j; i < min(i1, j + 32); ++i) stay |= r.keeps(r.s[i], r.lo + i) ? 1u << (i - j) : 0u;
+        for (; stay; stay &= stay - 1) s += r.weight(r.s[j + __ffs(stay) - 1]);
+    }
     const u64 inc = warp_scan(s, lane);
     if (lane == 31) sm.warp[warp] = inc;
     __syncthreads();
@@ -438,8 +516,8 @@ int sample_rows(const SampleRows &a, cudaStream_t s) {
         return ERR_ARG;
     }
     const int stretch = ((a.V + parts - 1) / parts + 3) / 4 * 4;
-    int sh = 62;
-    while (sh > 0 && (a.V - 1) >> (62 - sh)) --sh;  // V weights of 2^sh stay below 2^62
+    int sh = 50;
+    while ((a.V - 1) >> (62 - sh)) --sh;  // V weights of 2^sh stay below 2^62
     static bool set = false;
     if (!set) {
         CG_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
