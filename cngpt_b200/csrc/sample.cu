@@ -44,6 +44,23 @@ constexpr int BORDER = 512;  // keys that are compared with one another
 
 __device__ __forceinline__ u64 make_key(uint32_t rank, int i) { return ((u64)rank << 32) | (0xFFFFFFFFu - (uint32_t)i); }
 
+// 2^(j / TABLE) from the Taylor series of e^x, to the last bit or two
+struct Pow2 {
+    double v[TABLE];
+    constexpr Pow2() : v() {
+        for (int j = 0; j < TABLE; ++j) {
+            const double x = 0.6931471805599453 * j / TABLE;
+            double term = 1.0, sum = 0.0;
+            for (int n = 1; n < 30; ++n) {
+                sum += term;
+                term *= x / n;
+            }
+            v[j] = sum;
+        }
+    }
+};
+__device__ const Pow2 pow2_table;
+
 struct Border {  // what a block has of the border's bin
     int count;
     u64 lowest, highest;
@@ -63,12 +80,15 @@ struct Smem {
     Border mine;
     float max_of[MAX_PARTS], min_of[MAX_PARTS];
     u64 sum_of[MAX_PARTS];
+    float bar_of[MAX_PARTS];
     int first_of[MAX_PARTS];
     uint32_t fine_lo[NT], fine_hi[NT];
     short list_of[BORDER];
     int few;
     u64 warp[WARPS];
     float fwarp[2][WARPS];
+    float bar;
+    __align__(16) float own[NT];
     int bin;
     u64 above, cut;
 };
@@ -77,7 +97,7 @@ struct Row {
     const float *s;  // the block's stretch in shared memory
     int n, lo, per;  // its length, the index of its first token, tokens of a thread (odd: no bank conflicts)
     float mx;
-    double m, it;    // maximum, 1 / temperature
+    double m, t, it; // maximum, temperature, 1 / temperature
     double c;        // TABLE log2(e) / temperature
     int sh;
     const double *table;
@@ -85,6 +105,17 @@ struct Row {
     int cut_index;   // the ones up to this index
 
     __device__ bool keeps(float x, int i) const { return x > cut_at || (x == cut_at && i <= cut_index); }
+    // drops what weighs less than min_p: log w >= log min_p as a bound on the logit,
+    // rounded up to the next one
+    __device__ void least(float min_p) {
+        if (!(min_p > 0.0f)) return;
+        const double l = log(fmin(1.0, (double)min_p));
+        const float bound = l < 0.0 ? __double2float_ru(m + l * t) : mx;
+        if (bound > cut_at) {
+            cut_at = bound;
+            cut_index = 0x7FFFFFFF;
+        }
+    }
     __device__ float gap(float x) const { return x == mx ? 0.0f : mx - x; }
     __device__ void cut(u64 key) {
         cut_at = rank_value((uint32_t)(key >> 32));
@@ -123,6 +154,87 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
         if (lane >= o) v += u;
     }
     return v;
+}
+
+// the lowest and the highest over the block's threads, to sm.mine
+__device__ __forceinline__ void merge_span(u64 low, u64 high, Smem &sm) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+    }
+    if ((threadIdx.x & 31) == 0 && high) {
+        atomicMin(&sm.mine.lowest, low);
+        atomicMax(&sm.mine.highest, high);
+    }
+}
+
+// The lowest of sm.key[0, n) before which, in the ranking, the measure (1, or
+// sm.measure) and what lies `above` all of them stay below `limit`; above < limit
+// <= above + the sum of all. By the block.
+__device__ u64 border_cut(int n, u64 lowest, u64 highest, u64 above, u64 limit, bool weigh, Smem &sm) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // 256 bins of the keys' span first, one a thread
+    const int fine = max(0, 64 - __clzll((long long)(highest - lowest)) - 8);
+    auto fine_of = [&](u64 key) { return (int)((highest - key) >> fine); };
+    sm.fine_lo[tid] = sm.fine_hi[tid] = 0;
+    if (tid == 0) {
+        sm.cut = ~0ull;
+        sm.few = 0;
+    }
+    __syncthreads();
+    for (int e = tid; e < n; e += NT) {
+        const int f = fine_of(sm.key[e]);
+        const u64 w = weigh ? sm.measure[e] : 1;
+        const uint32_t l = (uint32_t)w, old = atomicAdd(&sm.fine_lo[f], l);
+        const uint32_t h = (uint32_t)(w >> 32) + (old + l < old ? 1u : 0u);
+        if (h) atomicAdd(&sm.fine_hi[f], h);
+    }
+    __syncthreads();
+    const u64 mine = ((u64)sm.fine_hi[tid] << 32) + sm.fine_lo[tid], scan = warp_scan(mine, lane);
+    if (lane == 31) sm.warp[warp] = scan;
+    __syncthreads();
+    u64 base = above + scan - mine;
+    for (int w = 0; w < warp; ++w) base += sm.warp[w];
+    if (base < limit && base + mine >= limit) {
+        sm.bin = tid;
+        sm.above = base;
+    }
+    __syncthreads();
+    for (int e = tid; e < n; e += NT)
+        if (fine_of(sm.key[e]) == sm.bin) sm.list_of[atomicAdd(&sm.few, 1)] = (short)e;
+    __syncthreads();
+    // each of those few against the others
+    u64 cut = ~0ull;
+    for (int e = tid; e < sm.few; e += NT) {
+        const u64 key = sm.key[sm.list_of[e]];
+        u64 b = sm.above;
+        for (int j = 0; j < sm.few; ++j) {
+            const int o = sm.list_of[j];
+            if (sm.key[o] > key) b += weigh ? sm.measure[o] : 1;
+        }
+        if (b < limit) cut = min(cut, key);
+    }
+    if (cut != ~0ull) atomicMin(&sm.cut, cut);
+    __syncthreads();
+    return sm.cut;
+}
+
+// every block's list to sm.key, block q's by warp q; lane q knows its length
+__device__ void gather(int n, int have, int parts, Smem &sm) {
+    auto cluster = coop::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int upto = have;
+#pragma unroll
+    for (int o = 1; o < MAX_PARTS; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (warp < parts) {
+        const int m = __shfl_sync(0xffffffffu, have, warp), at = __shfl_sync(0xffffffffu, upto, warp) - m;
+        const u64 *other = cluster.map_shared_rank(sm.list, warp);
+        for (int i = lane; i < m; i += 32) sm.key[at + i] = other[i];
+    }
 }
 
 // Raises r's cut to the border of the ranking at which the measure of the tokens
@@ -214,10 +326,7 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
             low = min(low, key);
             high = max(high, key);
         }
-        if (high) {
-            atomicMin(&sm.mine.lowest, low);
-            atomicMax(&sm.mine.highest, high);
-        }
+        merge_span(low, high, sm);
         cluster.sync();  // also: the bins have been read
         // every warp: lane q asks block q, then warp q fetches block q's keys
         int have = 0;
@@ -229,75 +338,109 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
             lowest = b->lowest;
             highest = b->highest;
         }
-        int upto = have;
 #pragma unroll
         for (int o = 1; o < MAX_PARTS; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
             lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, o));
             highest = max(highest, __shfl_xor_sync(0xffffffffu, highest, o));
         }
         lowest = __shfl_sync(0xffffffffu, lowest, 0);
         highest = __shfl_sync(0xffffffffu, highest, 0);
-        const int n = __shfl_sync(0xffffffffu, upto, MAX_PARTS - 1);
+        const int n = __reduce_add_sync(0xffffffffu, have);
         if (n <= BORDER) {
-            if (warp < parts) {
-                const int m = __shfl_sync(0xffffffffu, have, warp), at = __shfl_sync(0xffffffffu, upto, warp) - m;
-                const u64 *other = cluster.map_shared_rank(sm.list, warp);
-                for (int i = lane; i < m; i += 32) {
-                    const u64 key = other[i];
-                    sm.key[at + i] = key;
-                    if (WEIGHT) sm.measure[at + i] = r.weight(rank_value((uint32_t)(key >> 32)));
-                }
-            }
-            // the border among the keys: 256 bins of their span first, one a thread
-            const int fine = max(0, 64 - __clzll((long long)(highest - lowest)) - 8);
-            auto fine_of = [&](u64 key) { return (int)((highest - key) >> fine); };
-            sm.fine_lo[tid] = sm.fine_hi[tid] = 0;
-            if (tid == 0) {
-                sm.cut = ~0ull;
-                sm.few = 0;
-            }
+            gather(n, have, parts, sm);
             __syncthreads();
-            for (int e = tid; e < n; e += NT) {
-                const int f = fine_of(sm.key[e]);
-                const u64 w = WEIGHT ? sm.measure[e] : 1;
-                const uint32_t l = (uint32_t)w, old = atomicAdd(&sm.fine_lo[f], l);
-                const uint32_t h = (uint32_t)(w >> 32) + (old + l < old ? 1u : 0u);
-                if (h) atomicAdd(&sm.fine_hi[f], h);
-            }
+            if (WEIGHT)
+                for (int e = tid; e < n; e += NT) sm.measure[e] = r.weight(rank_value((uint32_t)(sm.key[e] >> 32)));
             __syncthreads();
-            const u64 mine = ((u64)sm.fine_hi[tid] << 32) + sm.fine_lo[tid], scan = warp_scan(mine, lane);
-            if (lane == 31) sm.warp[warp] = scan;
-            __syncthreads();
-            u64 base = above + scan - mine;
-            for (int w = 0; w < warp; ++w) base += sm.warp[w];
-            if (base < limit && base + mine >= limit) {
-                sm.bin = tid;
-                sm.above = base;
-            }
-            __syncthreads();
-            for (int e = tid; e < n; e += NT)
-                if (fine_of(sm.key[e]) == sm.bin) sm.list_of[atomicAdd(&sm.few, 1)] = (short)e;
-            __syncthreads();
-            // each of those few against the others
-            u64 cut = ~0ull;
-            for (int e = tid; e < sm.few; e += NT) {
-                const u64 key = sm.key[sm.list_of[e]];
-                u64 b = sm.above;
-                for (int j = 0; j < sm.few; ++j) {
-                    const int o = sm.list_of[j];
-                    if (sm.key[o] > key) b += WEIGHT ? sm.measure[o] : 1;
-                }
-                if (b < limit) cut = min(cut, key);
-            }
-            if (cut != ~0ull) atomicMin(&sm.cut, cut);
-            __syncthreads();
-            r.cut(sm.cut);
+            r.cut(border_cut(n, lowest, highest, above, limit, WEIGHT, sm));
             return;
         }
         // 10 bits of the span of the keys that are left
         shift = max(0, 64 - __clzll((long long)(highest - lowest)) - 10);
+    }
+}
+
+// The draw among sm.key[0, n), which hold the k first of the ranking, by one block.
+template <class Put>
+__device__ void draw_brief(Row &r, int n, int k, float p, float min_p, float u, Smem &sm, Put put) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto logit = [&](int e) { return rank_value((uint32_t)(sm.key[e] >> 32)); };
+    auto index = [&](int e) { return (int)(0xFFFFFFFFu - (uint32_t)sm.key[e]); };
+    auto span = [&](u64 &lowest, u64 &highest) {
+        if (tid == 0) sm.mine = {0, ~0ull, 0};
+        __syncthreads();
+        lowest = ~0ull;
+        highest = 0;
+        for (int e = tid; e < n; e += NT) {
+            lowest = min(lowest, sm.key[e]);
+            highest = max(highest, sm.key[e]);
+        }
+        merge_span(lowest, highest, sm);
+        __syncthreads();
+        lowest = sm.mine.lowest;
+        highest = sm.mine.highest;
+    };
+    auto sum = [&](u64 v) {
+        v = warp_scan(v, lane);
+        __syncthreads();
+        if (lane == 31) sm.warp[warp] = v;
+        __syncthreads();
+        v = 0;
+        for (int w = 0; w < WARPS; ++w) v += sm.warp[w];
+        return v;
+    };
+    u64 lowest, highest;
+    span(lowest, highest);
+    if (n > k) r.cut(border_cut(n, lowest, highest, 0, (u64)k, false, sm));
+    u64 s = 0;
+    for (int e = tid; e < n; e += NT) s += sm.measure[e] = r.keeps(logit(e), index(e)) ? r.weight(logit(e)) : 0;
+    u64 total = sum(s);
+    if (p < 1.0f) {
+        const u64 limit = max(1ull, (u64)ceil((double)p * (double)total));
+        if (limit < total) r.cut(border_cut(n, lowest, highest, 0, limit, true, sm));
+    }
+    r.least(min_p);
+    // those that stay, close together: index and weight
+    int *at = (int *)sm.fine_lo;
+    u64 *weight = sm.list;
+    if (tid == 0) sm.few = 0;
+    s = 0;
+    for (int e = tid; e < n; e += NT)
+        if (sm.measure[e] && r.keeps(logit(e), index(e))) s += sm.measure[e];
+    total = sum(s);
+    for (int e = tid; e < n; e += NT)
+        if (sm.measure[e] && r.keeps(logit(e), index(e))) {
+            const int j = atomicAdd(&sm.few, 1);  // at most k <= NT
+            at[j] = index(e);
+            weight[j] = sm.measure[e];
+            sm.list_of[j] = (short)e;
+        }
+    __syncthreads();
+    n = sm.few;
+    const u64 target = u < 1.0f ? min(total - 1, (u64)fmax(0.0, (double)u * (double)total)) : total - 1;
+    const double whole = ldexp((double)total, -r.sh);
+    if (target == 0 && u > 0.0f) {  // below one part: the weights as they are, see sample_kernel
+        if (tid != 0) return;
+        double c = 0.0;
+        for (int last = -1, left = n;; --left) {
+            int e = -1;  // the next one in index order
+            for (int j = 0; j < n; ++j)
+                if (at[j] > last && (e < 0 || at[j] < at[e])) e = j;
+            last = at[e];
+            const double y = r.exponent(logit(sm.list_of[e]));
+            c += exp(y);
+            if (c > (double)u * whole || left == 1) {
+                put(last, (float)(y - log(whole)));
+                return;
+            }
+        }
+    }
+    for (int e = tid; e < n; e += NT) {
+        u64 before = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) before += at[j] < at[e] ? weight[j] : 0;
+        if (before <= target && before + weight[e] > target)
+            put(at[e], (float)(r.exponent(logit(sm.list_of[e])) - log(whole)));
     }
 }
 
@@ -331,7 +474,7 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     const float T = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
     const float min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[at];
     const int k = a.top_k ? a.top_k[row] : 0;
-    if (tid < TABLE) sm.table[tid] = exp2((double)tid / TABLE);
+    if (tid < TABLE) sm.table[tid] = pow2_table.v[tid];
     auto put = [&](int token, float logprob) {
         a.tokens[at] = token;
         if (a.next) a.next[row] = max(token, 0);
@@ -354,26 +497,46 @@ sample_kernel(SampleRows a, int stretch, int sh) {
         look(v.w);
     }
     if (odd >= 0) look(r.s[odd]);
+    // a bar for a short top-k: of the threads' maxima the one that ceil(k / blocks)
+    // reach, the lowest over the blocks; k tokens reach it
+    const bool brief = k > 0 && k <= BORDER / 2 && T > 0.0f && p > 0.0f;
+    const float own = mx;  // of this thread
     mx = warp_max(mx);
     mn = -warp_max(-mn);
     if (lane == 0) {
         sm.fwarp[0][warp] = mx;
         sm.fwarp[1][warp] = mn;
+        if (warp == 0) sm.mine = {0, ~0ull, 0};
     }
+    sm.own[tid] = own;
     __syncthreads();
     for (int w = 0; w < WARPS; ++w) {
         mx = fmaxf(mx, sm.fwarp[0][w]);
         mn = fminf(mn, sm.fwarp[1][w]);
     }
+    if (brief) {
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < NT; j += 4) {
+            const float4 v = *(const float4 *)(sm.own + j);
+            rank += (v.x > own || (v.x == own && j < tid)) + (v.y > own || (v.y == own && j + 1 < tid)) +
+                    (v.z > own || (v.z == own && j + 2 < tid)) + (v.w > own || (v.w == own && j + 3 < tid));
+        }
+        if (rank == (k + parts - 1) / parts - 1) sm.bar = own;  // exactly one thread
+        __syncthreads();
+    }
+    float bar = brief ? sm.bar : -INFINITY;
     cluster.barrier_wait();
     if (tid < parts) {
         *cluster.map_shared_rank(&sm.max_of[part], tid) = mx;
         *cluster.map_shared_rank(&sm.min_of[part], tid) = mn;
+        *cluster.map_shared_rank(&sm.bar_of[part], tid) = bar;
     }
     cluster.sync();
     for (int q = 0; q < parts; ++q) {
         mx = fmaxf(mx, sm.max_of[q]);
         mn = fminf(mn, sm.min_of[q]);
+        bar = fminf(bar, sm.bar_of[q]);
     }
     if (mx == -INFINITY) {  // the same in every block, as all that follows
         if (part == 0 && tid == 0) put(-1, -INFINITY);
@@ -401,20 +564,48 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     }
     r.mx = mx;
     r.m = (double)mx;
-    r.it = 1.0 / (double)T;
+    r.t = (double)T;
+    r.it = 1.0 / r.t;
     r.c = TABLE * 1.4426950408889634 * r.it;
     r.cut_at = -INFINITY;
     r.cut_index = -1;
+    if (bar > -INFINITY) {
+        // A short top-k: the tokens that reach the bar, some 2 k, decide alone.
+        if (own >= bar) {
+            auto check = [&](float v, int i) {
+                if (v >= bar) {
+                    const int e = atomicAdd(&sm.mine.count, 1);
+                    if (e < BORDER) sm.list[e] = make_key(rank_key(v), r.lo + i);
+                }
+            };
+            if (odd >= 0) check(r.s[odd], odd);
+#pragma unroll 2
+            for (int q = tid; q < quads; q += NT) {
+                const float4 v = s4[q];
+                if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bar) {
+                    check(v.x, head + 4 * q);
+                    check(v.y, head + 4 * q + 1);
+                    check(v.z, head + 4 * q + 2);
+                    check(v.w, head + 4 * q + 3);
+                }
+            }
+        }
+        cluster.sync();
+        const int have = lane < parts ? cluster.map_shared_rank(&sm.mine, lane)->count : 0;
+        const int n = __reduce_add_sync(0xffffffffu, have);
+        if (n <= BORDER) {
+            if (part == 0) gather(n, have, parts, sm);
+            cluster.sync();  // the others' keys have been read
+            if (part == 0) draw_brief(r, n, k, p, min_p, u, sm, put);
+            return;
+        }
+        // too many equal logits: the general way
+    }
     // bins over the row's span, at most 64 wide (an outlier would stretch them)
     const float scale = mn < mx ? fminf((float)BINS / fminf(mx - mn, 64.0f), 1e30f) : 0.0f;
     if (k > 0 && k < a.V) cut_ranking<false>(r, scale, (u64)k, 0.0, sm);
     if (p < 1.0f) cut_ranking<true>(r, scale, 0, (double)p, sm);
-    if (min_p > 0.0f) {
-        // log w >= log min_p as a bound on the logit, rounded up to the next one
-        const double least = log(fmin(1.0, (double)min_p));
-        const float bound = least < 0.0 ? __double2float_ru(r.m + least * (double)T) : mx;
-        if (bound > r.cut_at) r.cut(make_key(rank_key(bound), 0x7FFFFFFF));
-    }
+    r.least(min_p);
 
     // cumulative weights in index order: threads, warps, blocks
     auto drawn = [&](int i) -> u64 {
