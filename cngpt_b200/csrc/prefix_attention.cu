@@ -35,8 +35,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// not volatile: independent products may be interleaved
 __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -71,14 +72,19 @@ struct Parts {  // the triples, [stretch][B * H]
 
 // ------------------------------------------------------------------ prefix
 constexpr int TK = 64;       // keys of a tile
-constexpr int PWARPS = 8;
 
-template <int HSP>
+template <int HSP, int RG>
 struct PrefixCfg {
+    // key groups: 8 warps up to two row groups, four warps a row group beyond
+    static constexpr int KG = RG == 1 ? 8 : 4, WARPS = RG * KG, KW = TK / KG;
+    static constexpr bool QREG = RG <= 2 && HSP <= 64;  // fragments of Q in registers, else in shared memory
+    static constexpr int QBUF = QREG ? 0 : 16 * RG * HSP * 2;
     static constexpr int LDK = HSP + 4;  // pitches without bank conflicts for ldmatrix rows and
     static constexpr int LDV = HSP + 8;  // for column-wise reads of four rows
     static constexpr int STAGE = TK * (LDK + LDV);
     static constexpr int STAGES = HSP <= 64 ? 4 : HSP <= 128 ? 2 : 1;
+    static constexpr int JOIN = KG * 16 * RG * (HSP + 2);
+    static constexpr int FLOATS = (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN) + QBUF;
 };
 
 // Block: 16 RG query rows of a key/value head against `chunk` keys. Warp (rg, kg)
@@ -88,11 +94,11 @@ struct PrefixCfg {
 // own accumulator, and P V starts a fresh accumulator in every tile that is
 // added in fp32, since the tensor core truncates as it accumulates.
 template <int HSP, int RG, bool SPLIT>
-__global__ void __launch_bounds__(PWARPS * 32, 1)
+__global__ void __launch_bounds__(PrefixCfg<HSP, RG>::WARPS * 32, 1)
 prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
-    using Cfg = PrefixCfg<HSP>;
-    constexpr int KG = PWARPS / RG, KW = TK / KG, NK = KW / 8, KK = HSP / 8, ND = HSP / 8;
-    constexpr int NT = PWARPS * 32;
+    using Cfg = PrefixCfg<HSP, RG>;
+    constexpr int KG = Cfg::KG, KW = Cfg::KW, NK = KW / 8, KK = HSP / 8, ND = HSP / 8;
+    constexpr int NT = Cfg::WARPS * 32;
     extern __shared__ float sm[];
     pdl_trigger();
     const int split = blockIdx.x % w.n_pre, tile = blockIdx.x / w.n_pre % n_tiles, hk = blockIdx.x / w.n_pre / n_tiles;
@@ -108,8 +114,9 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
         const int k0 = k_lo + i * TK;
         if (vec) {
 #pragma unroll
-            for (int c = 0; c < TK * (HSP / 4) / NT; ++c) {
+            for (int c = 0; c < (TK * (HSP / 4) + NT - 1) / NT; ++c) {
                 const int e = c * NT + threadIdx.x, r = e / (HSP / 4), d = e % (HSP / 4) * 4;
+                if (TK * (HSP / 4) % NT && r >= TK) break;
                 const bool ok = k0 + r < k_hi && d < hs;
                 const long at = ok ? (long)(k0 + r) * a.ldp + d : 0;
                 cp_async16(dk + r * Cfg::LDK + d, kbase + at, ok);
@@ -132,23 +139,35 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    // the rows' fragments of Q scale log2(e), split, in registers
-    uint32_t qh[KK][4], ql[KK][4];
+    // the rows' fragments of Q scale log2(e), split
+    constexpr int QK = Cfg::QREG ? KK : 1;
+    uint32_t qh[QK][4], ql[QK][4];
+    uint4 *sq = (uint4 *)(sm + Cfg::FLOATS - Cfg::QBUF) + rg * KK * 64 + lane;  // [KK][hi, lo][32 lanes] of the row group
     {
         const float sc = a.scale * LOG2E;
         const int r0 = tile * 16 * RG + rg * 16 + g, r1 = r0 + 8;
         auto row = [&](int r) { return a.q + (long)(r / G) * a.ldq + (long)(hk * G + r % G) * hs; };
         const float *p0 = row(min(r0, R - 1)), *p1 = row(min(r1, R - 1));
-#pragma unroll
-        for (int k = 0; k < KK; ++k)
+        auto fragment = [&](int k, uint32_t (&h)[4], uint32_t (&l)[4]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int d = 8 * k + t + (e >> 1) * 4;
                 const bool ok = d < hs && ((e & 1) ? r1 : r0) < R;
                 const float v = ok ? ((e & 1) ? p1 : p0)[d] * sc : 0.0f;
-                if constexpr (SPLIT) split_tf32(v, qh[k][e], ql[k][e]);
-                else qh[k][e] = __float_as_uint(v);
+                if constexpr (SPLIT) split_tf32(v, h[e], l[e]);
+                else h[e] = l[e] = __float_as_uint(v);
             }
+        };
+        if constexpr (Cfg::QREG) {
+#pragma unroll
+            for (int k = 0; k < KK; ++k) fragment(k, qh[k], ql[k]);
+        } else {
+            for (int k = kg; k < KK; k += KG) {  // the first tile's barrier shows them to the group
+                fragment(k, qh[0], ql[0]);
+                sq[k * 64] = make_uint4(qh[0][0], qh[0][1], qh[0][2], qh[0][3]);
+                sq[k * 64 + 32] = make_uint4(ql[0][0], ql[0][1], ql[0][2], ql[0][3]);
+            }
+        }
     }
 
     float o[ND][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -170,22 +189,40 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
             const float *kr = sk + (kg * KW + ((lane & 7) >> 1) + 4 * (lane & 1)) * Cfg::LDK + (lane >> 3) * 4;
 #pragma unroll
             for (int k = 0; k < KK; k += 2) {
+                uint32_t b[NK][4];
 #pragma unroll
-                for (int j = 0; j < NK; ++j) {
-                    uint32_t b[4];
-                    ldsm4(b, kr + j * 8 * Cfg::LDK + k * 8);
+                for (int j = 0; j < NK; ++j) ldsm4(b[j], kr + j * 8 * Cfg::LDK + k * 8);
+                // the products of one kind over all keys in a row: none waits for the one before
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        if constexpr (SPLIT) {
-                            uint32_t h0, h1, l0, l1;
-                            split_tf32(__uint_as_float(b[2 * u]), h0, l0);
-                            split_tf32(__uint_as_float(b[2 * u + 1]), h1, l1);
-                            mma8(sl[j], ql[k + u], h0, h1);
-                            mma8(sl[j], qh[k + u], l0, l1);
-                            mma8(s[j], qh[k + u], h0, h1);
-                        } else {
-                            mma8(s[j], qh[k + u], b[2 * u], b[2 * u + 1]);
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t ah[4], al[4];
+                    if constexpr (Cfg::QREG) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            ah[e] = qh[k + u][e];
+                            al[e] = ql[k + u][e];
                         }
+                    } else {
+                        const uint4 x = sq[(k + u) * 64], y = SPLIT ? sq[(k + u) * 64 + 32] : x;
+                        ah[0] = x.x, ah[1] = x.y, ah[2] = x.z, ah[3] = x.w;
+                        al[0] = y.x, al[1] = y.y, al[2] = y.z, al[3] = y.w;
+                    }
+                    if constexpr (SPLIT) {
+                        uint32_t h[NK][2], l[NK][2];
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) {
+                            split_tf32(__uint_as_float(b[j][2 * u]), h[j][0], l[j][0]);
+                            split_tf32(__uint_as_float(b[j][2 * u + 1]), h[j][1], l[j][1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) mma8(sl[j], al, h[j][0], h[j][1]);
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) mma8(s[j], ah, h[j][0], h[j][1]);
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) mma8(sl[j], ah, l[j][0], l[j][1]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NK; ++j) mma8(s[j], ah, b[j][2 * u], b[j][2 * u + 1]);
                     }
                 }
             }
@@ -221,24 +258,40 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
                 }
             const float *vr = sv + (kg * KW + t) * Cfg::LDV + g;
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-                float acc[4] = {}, acl[4] = {};
+            for (int n0 = 0; n0 < ND; n0 += 4) {
+                float acc[4][4] = {}, acl[4][4] = {};
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
-                    const float v0 = vr[j * 8 * Cfg::LDV + n * 8], v1 = vr[(j * 8 + 4) * Cfg::LDV + n * 8];
+                    float v[4][2];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        v[n][0] = vr[j * 8 * Cfg::LDV + (n0 + n) * 8];
+                        v[n][1] = vr[(j * 8 + 4) * Cfg::LDV + (n0 + n) * 8];
+                    }
                     if constexpr (SPLIT) {
-                        uint32_t h0, h1, l0, l1;
-                        split_tf32(v0, h0, l0);
-                        split_tf32(v1, h1, l1);
-                        mma8(acl, pl[j], h0, h1);
-                        mma8(acl, ph[j], l0, l1);
-                        mma8(acc, ph[j], h0, h1);
+                        uint32_t h[4][2], l[4][2];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            split_tf32(v[n][0], h[n][0], l[n][0]);
+                            split_tf32(v[n][1], h[n][1], l[n][1]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) mma8(acl[n], pl[j], h[n][0], h[n][1]);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) mma8(acc[n], ph[j], h[n][0], h[n][1]);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) mma8(acl[n], ph[j], l[n][0], l[n][1]);
                     } else {
-                        mma8(acc, ph[j], __float_as_uint(v0), __float_as_uint(v1));
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            mma8(acc[n], ph[j], __float_as_uint(v[n][0]), __float_as_uint(v[n][1]));
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][e] = fmaf(o[n][e], c[e >> 1], acc[e] + acl[e]);
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[n0 + n][e] = fmaf(o[n0 + n][e], c[e >> 1], acc[n][e] + acl[n][e]);
             }
         }
         if constexpr (Cfg::STAGES == 1) {
@@ -464,7 +517,14 @@ __global__ void shared_advance_kernel(int *ctr, int *suffix_len, int n) {
 }
 
 // ------------------------------------------------------------- the launches
-int row_groups(long R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+// Rows of 16 that a block takes: up to 64 rows read a tile once. Above 128
+// dimensions the tile and the queries of more than 32 rows do not fit.
+int row_groups(long R, int hs) {
+    if (R <= 16) return 1;
+    if (R <= 32 || hs > 128) return 2;
+    // 48 rows a block where that takes as few blocks as 64 would
+    return (R + 47) / 48 == (R + 63) / 64 ? 3 : 4;
+}
 
 // Stretches: the prefix is cut so that its blocks fill the SMs about once (one
 // block an SM), but not below one tile; the suffixes into what one block loads
@@ -472,7 +532,7 @@ int row_groups(long R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 Parts plan(int B, int H, int Hk, int hs, int P, int S) {
     Parts w{};
     const long R = (long)B * (H / Hk);
-    const int rg = row_groups(R);
+    const int rg = row_groups(R, hs);
     if (P > 0) {
         const long n_tiles = (R + 16 * rg - 1) / (16 * rg), tiles = (P + TK - 1) / TK;
         const long want = std::max<long>(1, 148 / std::max<long>(1, Hk * n_tiles));
@@ -509,9 +569,9 @@ int launch_pdl(K kernel, long grid, int threads, size_t smem, bool chained, cuda
 
 template <int HSP, int RG, bool SPLIT>
 int launch_prefix(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
-    using Cfg = PrefixCfg<HSP>;
-    constexpr size_t join = (size_t)(PWARPS / RG) * 16 * RG * (HSP + 2);
-    constexpr size_t smem = std::max((size_t)Cfg::STAGES * Cfg::STAGE, join) * sizeof(float);
+    using Cfg = PrefixCfg<HSP, RG>;
+    constexpr size_t smem = (size_t)Cfg::FLOATS * sizeof(float);
+    static_assert(smem <= 227 * 1024, "shared memory of a block");
     static bool set = false;
     if (!set) {
         CG_CUDA(cudaFuncSetAttribute(prefix_part_kernel<HSP, RG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -520,16 +580,19 @@ int launch_prefix(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
     }
     const long R = (long)a.B * (a.H / a.Hk), n_tiles = (R + 16 * RG - 1) / (16 * RG);
     const bool vec = a.hs % 4 == 0 && a.ldp % 4 == 0 && ((uintptr_t)a.pk | (uintptr_t)a.pv) % 16 == 0;
-    return launch_pdl(prefix_part_kernel<HSP, RG, SPLIT>, (long)w.n_pre * n_tiles * a.Hk, PWARPS * 32, smem, false, s, a, w,
+    return launch_pdl(prefix_part_kernel<HSP, RG, SPLIT>, (long)w.n_pre * n_tiles * a.Hk, Cfg::WARPS * 32, smem, false, s, a, w,
                       (int)n_tiles, vec);
 }
 
 template <int HSP, bool SPLIT>
 int dispatch_rows(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
-    const int rg = row_groups((long)a.B * (a.H / a.Hk));
+    const int rg = row_groups((long)a.B * (a.H / a.Hk), a.hs);
     if (rg == 1) return launch_prefix<HSP, 1, SPLIT>(a, w, s);
-    if (rg == 2) return launch_prefix<HSP, 2, SPLIT>(a, w, s);
-    return launch_prefix<HSP, 4, SPLIT>(a, w, s);
+    if constexpr (HSP <= 128) {
+        if (rg == 3) return launch_prefix<HSP, 3, SPLIT>(a, w, s);
+        if (rg == 4) return launch_prefix<HSP, 4, SPLIT>(a, w, s);
+    }
+    return launch_prefix<HSP, 2, SPLIT>(a, w, s);
 }
 
 template <bool SPLIT>
