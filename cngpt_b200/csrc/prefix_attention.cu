@@ -43,12 +43,25 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t *a, uint32_t 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo in two tf32 numbers: hi is x rounded to 11 significant bits (half
-// away from zero, on the bit pattern), lo the exact rest, rounded the same way
-// by the tensor core's cut of the added half step. The pair is x to 2^-23.
+// d = a b: the first product of a sum
+__device__ __forceinline__ void mma8_first(float (&d)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// x = hi + lo in two tf32 numbers. Rounded: hi is x to 11 significant bits (half
+// away from zero, on the bit pattern), lo the exact rest with half a step added
+// before the tensor core cuts it to 11 bits: x to 2^-23. For what is loaded anew
+// for every tile (K, V) both are cut, two instructions for four: x to 2^-21,
+// 2^-22 on average and towards zero, so a score or an output shrinks by 1e-7.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+}
+__device__ __forceinline__ void cut_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const float *p) {
@@ -64,8 +77,9 @@ __device__ __forceinline__ void cp_async4(float *dst, const float *src, bool ok)
 }
 
 struct Parts {  // the triples, [stretch][B * H]
-    float *o;     // [hs] each
+    float *o;     // [pitch] each, pitch = hs rounded up to 4
     float2 *ml;
+    int pitch;
     int n_pre, chunk;      // prefix stretches and their keys
     int n_suf, suf_chunk;  // suffix stretches (of the capacity) and their keys
 };
@@ -82,7 +96,7 @@ struct PrefixCfg {
     static constexpr int LDK = HSP + 4;  // pitches without bank conflicts for ldmatrix rows and
     static constexpr int LDV = HSP + 8;  // for column-wise reads of four rows
     static constexpr int STAGE = TK * (LDK + LDV);
-    static constexpr int STAGES = HSP <= 64 ? 4 : HSP <= 128 ? 2 : 1;
+    static constexpr int STAGES = HSP <= 64 ? 3 : HSP <= 128 ? 2 : 1;
     static constexpr int JOIN = KG * 16 * RG * (HSP + 2);
     static constexpr int FLOATS = (STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN) + QBUF;
 };
@@ -90,11 +104,12 @@ struct PrefixCfg {
 // Block: 16 RG query rows of a key/value head against `chunk` keys. Warp (rg, kg)
 // takes rows 16 rg .. 16 rg + 15 and the keys [KW kg, KW kg + KW) of every tile,
 // with its own running maximum, so warps meet only where tiles are exchanged.
-// Products are split in three (lo*hi + hi*lo + hi*hi); the small two have their
-// own accumulator, and P V starts a fresh accumulator in every tile that is
-// added in fp32, since the tensor core truncates as it accumulates.
+// Products are split in three (lo*hi + hi*lo + hi*hi). The tensor core truncates
+// as it accumulates, so the small products of a score have their own accumulator
+// and P V starts a fresh one in every tile, which is added in fp32.
 template <int HSP, int RG, bool SPLIT>
-__global__ void __launch_bounds__(PrefixCfg<HSP, RG>::WARPS * 32, 1)
+// 48 rows keep 128 registers a thread, so that a suffix block fits beside them
+__global__ void __launch_bounds__(RG == 3 ? 512 : PrefixCfg<HSP, RG>::WARPS * 32, 1)
 prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
     using Cfg = PrefixCfg<HSP, RG>;
     constexpr int KG = Cfg::KG, KW = Cfg::KW, NK = KW / 8, KK = HSP / 8, ND = HSP / 8;
@@ -182,7 +197,7 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
         const float *sk = sm + (i % Cfg::STAGES) * Cfg::STAGE, *sv = sk + TK * Cfg::LDK;
         const int valid = min(TK, k_hi - k_lo - i * TK);
         if (kg * KW < valid) {
-            float s[NK][4] = {}, sl[NK][4] = {};
+            float s[NK][4], sl[NK][4];
             // accumulator column n of a group of 8 holds key (n >> 1) + 4 (n & 1),
             // so that a thread's two columns are the keys t and t + 4 of the A
             // fragment that the same registers form in P V
@@ -211,30 +226,41 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
                         uint32_t h[NK][2], l[NK][2];
 #pragma unroll
                         for (int j = 0; j < NK; ++j) {
-                            split_tf32(__uint_as_float(b[j][2 * u]), h[j][0], l[j][0]);
-                            split_tf32(__uint_as_float(b[j][2 * u + 1]), h[j][1], l[j][1]);
+                            cut_tf32(__uint_as_float(b[j][2 * u]), h[j][0], l[j][0]);
+                            cut_tf32(__uint_as_float(b[j][2 * u + 1]), h[j][1], l[j][1]);
                         }
 #pragma unroll
-                        for (int j = 0; j < NK; ++j) mma8(sl[j], al, h[j][0], h[j][1]);
+                        for (int j = 0; j < NK; ++j)
+                            k + u ? mma8(sl[j], al, h[j][0], h[j][1]) : mma8_first(sl[j], al, h[j][0], h[j][1]);
 #pragma unroll
-                        for (int j = 0; j < NK; ++j) mma8(s[j], ah, h[j][0], h[j][1]);
+                        for (int j = 0; j < NK; ++j)
+                            k + u ? mma8(s[j], ah, h[j][0], h[j][1]) : mma8_first(s[j], ah, h[j][0], h[j][1]);
 #pragma unroll
                         for (int j = 0; j < NK; ++j) mma8(sl[j], ah, l[j][0], l[j][1]);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < NK; ++j) mma8(s[j], ah, b[j][2 * u], b[j][2 * u + 1]);
+                        for (int j = 0; j < NK; ++j)
+                            k + u ? mma8(s[j], ah, b[j][2 * u], b[j][2 * u + 1])
+                                  : mma8_first(s[j], ah, b[j][2 * u], b[j][2 * u + 1]);
                     }
                 }
             }
             float mx[2] = {m[0], m[1]};
+            if (SPLIT)
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][e] += sl[j][e];
+            if (valid < TK)  // the last tile
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (kg * KW + j * 8 + t + (e & 1) * 4 >= valid) s[j][e] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NK; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = kg * KW + j * 8 + t + (e & 1) * 4;
-                    s[j][e] = key < valid ? s[j][e] + sl[j][e] : -INFINITY;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
-                }
+                for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[j][e]);
             float c[2], ref[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -259,7 +285,7 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
             const float *vr = sv + (kg * KW + t) * Cfg::LDV + g;
 #pragma unroll
             for (int n0 = 0; n0 < ND; n0 += 4) {
-                float acc[4][4] = {}, acl[4][4] = {};
+                float acc[4][4];  // the tile's own sum, the small products first
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {
                     float v[4][2];
@@ -272,26 +298,29 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
                         uint32_t h[4][2], l[4][2];
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
-                            split_tf32(v[n][0], h[n][0], l[n][0]);
-                            split_tf32(v[n][1], h[n][1], l[n][1]);
+                            cut_tf32(v[n][0], h[n][0], l[n][0]);
+                            cut_tf32(v[n][1], h[n][1], l[n][1]);
                         }
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) mma8(acl[n], pl[j], h[n][0], h[n][1]);
+                        for (int n = 0; n < 4; ++n)
+                            j ? mma8(acc[n], pl[j], h[n][0], h[n][1]) : mma8_first(acc[n], pl[j], h[n][0], h[n][1]);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) mma8(acc[n], ph[j], l[n][0], l[n][1]);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) mma8(acc[n], ph[j], h[n][0], h[n][1]);
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) mma8(acl[n], ph[j], l[n][0], l[n][1]);
                     } else {
 #pragma unroll
-                        for (int n = 0; n < 4; ++n)
-                            mma8(acc[n], ph[j], __float_as_uint(v[n][0]), __float_as_uint(v[n][1]));
+                        for (int n = 0; n < 4; ++n) {
+                            const uint32_t v0 = __float_as_uint(v[n][0]), v1 = __float_as_uint(v[n][1]);
+                            j ? mma8(acc[n], ph[j], v0, v1) : mma8_first(acc[n], ph[j], v0, v1);
+                        }
                     }
                 }
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        o[n0 + n][e] = fmaf(o[n0 + n][e], c[e >> 1], acc[n][e] + acl[n][e]);
+                        o[n0 + n][e] = fmaf(o[n0 + n][e], c[e >> 1], acc[n][e]);
             }
         }
         if constexpr (Cfg::STAGES == 1) {
@@ -334,7 +363,7 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
             oo = fmaf(so[(k * 16 * RG + rr) * HSP + d], f, oo);
         }
         const long id = split * BH + (long)(r / G) * a.H + hk * G + r % G;
-        if (d < hs) w.o[id * hs + d] = oo;
+        if (d < hs) w.o[id * w.pitch + d] = oo;
         if (d == 0) w.ml[id] = make_float2(mm, ll);
     }
 }
@@ -343,7 +372,7 @@ prefix_part_kernel(PrefixAttn a, Parts w, int n_tiles, bool vec) {
 // Block: one sequence, one key/value head, one stretch of CH keys. LPK lanes hold
 // one key's row (NF float4 each), so a warp reads 32 / LPK whole rows at a time;
 // all K and V rows of the stretch are on their way before the first is used.
-constexpr int SWARPS = 8;
+constexpr int SWARPS = 4;
 
 template <int LPK, int NF>
 struct SuffixCfg {
@@ -365,7 +394,7 @@ __device__ __forceinline__ float4 row4(const float *p, int d, int hs, bool ok, b
 }
 
 template <int LPK, int NF>
-__global__ void __launch_bounds__(SWARPS * 32)
+__global__ void __launch_bounds__(SWARPS * 32, 4)
 suffix_part_kernel(PrefixAttn a, Parts w, bool vec) {
     using Cfg = SuffixCfg<LPK, NF>;
     __shared__ float so[SWARPS][LPK * 4 * NF];
@@ -454,7 +483,7 @@ suffix_part_kernel(PrefixAttn a, Parts w, bool vec) {
                 float oo = 0.0f;
 #pragma unroll
                 for (int x = 0; x < SWARPS; ++x) oo = fmaf(so[x][d], ex2(sml[x].x - r2), oo);
-                w.o[id * hs + d] = oo;
+                w.o[id * w.pitch + d] = oo;
             }
             if (threadIdx.x == 0) {
 #pragma unroll
@@ -467,48 +496,67 @@ suffix_part_kernel(PrefixAttn a, Parts w, bool vec) {
 }
 
 // -------------------------------------------------------------------- join
-constexpr int JWARPS = 4;
+constexpr int JT = 128, JBATCH = 4;
 
-__global__ void __launch_bounds__(JWARPS * 32)
-join_kernel(PrefixAttn a, Parts w) {
-    __shared__ float so[JWARPS][256];
-    __shared__ float sl[JWARPS];
+// Block: one query. Groups of `lp` threads (four dimensions each) take every JT / lp
+// -th stretch, JBATCH of them on their way at a time; the groups' triples are then
+// joined in order.
+__global__ void __launch_bounds__(JT)
+join_kernel(PrefixAttn a, Parts w, int lp) {
+    __shared__ float4 so[JT];
+    __shared__ float2 sml[JT];
     const long row = blockIdx.x, BH = (long)a.B * a.H;
     const int b = (int)(row / a.H), h = (int)(row % a.H), hs = a.hs;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sub = threadIdx.x / lp, li = threadIdx.x % lp, groups = JT / lp;
     const int len = a.S > 0 ? min(max(a.suffix_len[b], 0), a.S) : 0;
     const int n = w.n_pre + (len > 0 ? (len + w.suf_chunk - 1) / w.suf_chunk : 0);
+    const bool on = 4 * li < hs;
     pdl_wait();
-    float m = -INFINITY;
-    for (int s = lane; s < n; s += 32) m = fmaxf(m, w.ml[s * BH + row].x);
-    m = warp_max(m);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    // each warp joins every JWARPS-th stretch
-    float l = 0.0f, o[8] = {};
-    for (int s = warp; s < n; s += JWARPS) {
-        const float2 p = w.ml[s * BH + row];
-        const float f = ex2(p.x - ref);
-        l = fmaf(p.y, f, l);
-        const float *po = w.o + (s * BH + row) * hs;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = sub; s0 < n; s0 += JBATCH * groups) {
+        float2 p[JBATCH];
+        float4 v[JBATCH];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (lane + 32 * i < hs) o[i] = fmaf(po[lane + 32 * i], f, o[i]);
+        for (int j = 0; j < JBATCH; ++j) {
+            const int s = s0 + j * groups;
+            p[j] = s < n ? w.ml[s * BH + row] : make_float2(-INFINITY, 0.0f);
+            v[j] = s < n && on ? *(const float4 *)(w.o + (s * BH + row) * w.pitch + 4 * li) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float mx = m;
+#pragma unroll
+        for (int j = 0; j < JBATCH; ++j) mx = fmaxf(mx, p[j].x);
+        const float ref = mx == -INFINITY ? 0.0f : mx, c = ex2(m - ref);
+        m = mx;
+        l *= c;
+        o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+#pragma unroll
+        for (int j = 0; j < JBATCH; ++j) {
+            const float f = ex2(p[j].x - ref);
+            l = fmaf(p[j].y, f, l);
+            o = make_float4(fmaf(v[j].x, f, o.x), fmaf(v[j].y, f, o.y), fmaf(v[j].z, f, o.z), fmaf(v[j].w, f, o.w));
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < hs) so[warp][lane + 32 * i] = o[i];
-    if (lane == 0) sl[warp] = l;
+    so[threadIdx.x] = o;
+    if (li == 0) sml[sub] = make_float2(m, l);
     __syncthreads();
-    l = sl[0];
-#pragma unroll
-    for (int x = 1; x < JWARPS; ++x) l += sl[x];
-    const float inv = n > 0 ? 1.0f / l : 0.0f;
-    for (int d = threadIdx.x; d < hs; d += JWARPS * 32) {
-        float oo = so[0][d];
-#pragma unroll
-        for (int x = 1; x < JWARPS; ++x) oo += so[x][d];
-        a.out[b * a.ldo + (long)h * hs + d] = n > 0 ? oo * inv : 0.0f;
+    if (sub != 0 || !on) return;
+    m = -INFINITY;
+    for (int x = 0; x < groups; ++x) m = fmaxf(m, sml[x].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int x = 0; x < groups; ++x) {
+        const float f = ex2(sml[x].x - ref);
+        const float4 v = so[x * lp + li];
+        l = fmaf(sml[x].y, f, l);
+        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
     }
+    const float inv = n > 0 ? 1.0f / l : 0.0f, e[4] = {o.x, o.y, o.z, o.w};
+    float *out = a.out + b * a.ldo + (long)h * hs + 4 * li;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (4 * li + j < hs) out[j] = n > 0 ? e[j] * inv : 0.0f;
 }
 
 __global__ void shared_advance_kernel(int *ctr, int *suffix_len, int n) {
@@ -531,6 +579,7 @@ int row_groups(long R, int hs) {
 // at once.
 Parts plan(int B, int H, int Hk, int hs, int P, int S) {
     Parts w{};
+    w.pitch = (hs + 3) / 4 * 4;
     const long R = (long)B * (H / Hk);
     const int rg = row_groups(R, hs);
     if (P > 0) {
@@ -615,7 +664,7 @@ int shared_advance(int *ctr, int *suffix_len, int n, cudaStream_t s) {
 size_t prefix_attention_ws_bytes(int B, int H, int Hk, int hs, int P, int S) {
     const Parts w = plan(B, H, Hk, hs, P, S);
     const size_t rows = (size_t)(w.n_pre + w.n_suf) * B * H;
-    return (rows * hs * sizeof(float) + 15) / 16 * 16 + rows * sizeof(float2);
+    return rows * (w.pitch * sizeof(float) + sizeof(float2));
 }
 
 int prefix_attention(const PrefixAttn &a, void *ws, cudaStream_t s) {
@@ -623,7 +672,7 @@ int prefix_attention(const PrefixAttn &a, void *ws, cudaStream_t s) {
     Parts w = plan(a.B, a.H, a.Hk, a.hs, a.P, a.S);
     w.o = (float *)ws;
     const size_t rows = (size_t)(w.n_pre + w.n_suf) * a.B * a.H;
-    w.ml = (float2 *)((char *)ws + (rows * a.hs * sizeof(float) + 15) / 16 * 16);
+    w.ml = (float2 *)(w.o + rows * w.pitch);
     bool chained = false;
     if (w.n_pre > 0) {
         CG_TRY(precision() == PREC_TF32 ? dispatch_hs<false>(a, w, s) : dispatch_hs<true>(a, w, s));
@@ -640,7 +689,9 @@ int prefix_attention(const PrefixAttn &a, void *ws, cudaStream_t s) {
         else CG_TRY(go(suffix_part_kernel<32, 2>));
         chained = true;
     }
-    return launch_pdl(join_kernel, (long)a.B * a.H, JWARPS * 32, 0, chained, s, a, w);
+        int lp = 8;  // threads of a row in the join
+    while (4 * lp < a.hs) lp *= 2;
+    return launch_pdl(join_kernel, (long)a.B * a.H, JT, 0, chained, s, a, w, lp);
 }
 
 }  // namespace cg
