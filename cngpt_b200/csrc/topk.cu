@@ -53,8 +53,8 @@ struct Smem {
 // instructions of one warp take the place of some 5000 of all warps.
 constexpr int SMALL = 512;
 
+template <int PER>
 __device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
-    constexpr int PER = SMALL / 32;
     const int lane = threadIdx.x & 31;
     uint32_t key[PER], top = 0, bottom = 0xFFFFFFFFu;
 #pragma unroll
@@ -71,8 +71,10 @@ __device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
         int c = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) c += key[j] >= mid;
-        if (__reduce_add_sync(0xffffffffu, c) >= k) lo = mid;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= k) lo = mid;
         else hi = mid - 1;
+        if (c == k) break;  // just these; whether `lo` is one of them does not matter
     }
     int above = 0, equal = 0;
 #pragma unroll
@@ -109,7 +111,8 @@ __device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
     }
     if (lane == 0) {
         sm.count = k;
-        sm.low = lo;
+        // between NaN (0) and -inf lies no logit: k numbers, what follows has to exceed -inf
+        sm.low = lo == 0u ? 0u : max(lo, RANK_NEG_INF);
     }
 }
 
@@ -120,7 +123,11 @@ __device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
 __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (n <= SMALL) {
-        if (warp == 0) select_small(buf, n, k, sm);
+        if (warp == 0) {
+            if (n <= 128) select_small<4>(buf, n, k, sm);
+            else if (n <= 256) select_small<8>(buf, n, k, sm);
+            else select_small<SMALL / 32>(buf, n, k, sm);
+        }
         __syncthreads();
         return;
     }
@@ -231,7 +238,7 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
     const int trigger = max(2 * k, TRIGGER);
     bool all = true;  // fewer than k kept: every element is a candidate, NaN too
     float low = 0.0f;
-    if (k <= NT && chunks > 1) {
+    if (k <= NT) {
         // A first bar from the first chunk: each warp's ceil(k / warps)-th largest
         // of its lanes' maxima, the lowest of them. At least k elements of the
         // chunk reach it, so what lies below it cannot count, nor can an equal one

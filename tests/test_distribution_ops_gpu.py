@@ -272,6 +272,22 @@ def test_topk_ties_orders_and_special_values(lib, cuda, k):
     check_topk(lib, x, k)
 
 
+@pytest.mark.parametrize("tail", [0, 1, 3])
+def test_topk_numbers_after_nan(lib, cuda, tail):
+    """Rows of NaN with as many numbers as are asked for, and larger ones at the
+    very end: whatever was cut before must let those pass."""
+    V = 4096 + 100 + tail
+    x = np.full((3, V), NAN, np.float32)
+    x[:, [3, 700, 1500, 2222, 4000]] = [1.0, -2.0, 3.0, -INF, 5.0]
+    x[:, [4100, 4120, 4130, 4140, 4150]] = [0.5, -INF, 2.0, -3.0, 4.0]
+    if tail:
+        x[1, V - tail:] = 100.0 + np.arange(tail)
+        x[2, V - 1] = -INF
+    check_topk(lib, x, 10)
+    check_topk(lib, x, 9)
+    check_topk(lib, x, 12)
+
+
 def test_topk_many_rows(lib, cuda):
     check_topk(lib, logits(700, 3001, 11), 33)
 
