@@ -9,6 +9,13 @@
 // writing its gradient once is all that has to move (8 bytes a logit, 4 without
 // gradient), so a cluster of blocks keeps the row in its shared memory between
 // the pass that forms the sums and the pass that writes.
+//
+// On B200, 8192 x 50257 with both softmaxes and the gradient: 0.755 ms (4.4 TB/s, 67 %
+// of the copy rate); the loss of 1024 rows alone: 60 us (3.4 TB/s). What is left is the
+// latency of a row's phases (loads, two block barriers, one cluster barrier), which
+// four blocks an SM do not hide; the exponentials take half of the special-function
+// units' time. Smaller and larger blocks and stretches took 0.756 to 1.24 ms,
+// clusters that prefetch their next row 2.0 ms (the list's loads delay every row).
 #include <algorithm>
 #include <cmath>
 

@@ -14,7 +14,15 @@
 // weights over 1024 bins of max - l, whose prefix sums give the bin that the
 // border falls into; the few hundred keys of that bin are then compared with one
 // another. Where a bin holds more than that (runs of equal logits, outliers that
-// stretch the bins), it is cut again by the bits of its keys until it does not.
+// stretch the bins), it is cut again by the bits of its keys until it does not. A
+// short top-k needs none of this: some 2 k tokens reach a bar that the threads'
+// maxima give, and one block draws among them.
+//
+// On B200: 1 x 50257 with top-k and top-p 14.3 us, 64 rows with min-p 11 us, 32 rows
+// with settings of their own 33 us, 256 rows by top-p alone 122 us (reading them:
+// 7.9 us). The last is bound by the shared-memory atomics of the weights (30
+// cycles a warp: half of the time) and by the exponentials; summing the weights in
+// limbs without returned values took twice as long, 26 KB stretches half more.
 #include <algorithm>
 #include <cmath>
 
@@ -34,10 +42,7 @@ typedef unsigned long long u64;
 constexpr int NT = 256;
 constexpr int WARPS = NT / 32;
 constexpr int MAX_PARTS = 8;
-#ifndef SM_SLICE
-#define SM_SLICE 52
-#endif
-constexpr int SLICE_BYTES = SM_SLICE * 1024;  // of a row in a block's shared memory
+constexpr int SLICE_BYTES = 52 * 1024;  // of a row in a block's shared memory: three blocks an SM
 constexpr int BINS = 4 * NT;
 constexpr int TABLE = 64;    // entries 2^(j / 64) of the exponential
 constexpr int BORDER = 512;  // keys that are compared with one another
@@ -238,7 +243,7 @@ __device__ void gather(int n, int have, int parts, Smem &sm) {
 }
 
 // Raises r's cut to the border of the ranking at which the measure of the tokens
-// before (their number, or WEIGHT) reaches a limit: `k`, or the part `p` of the
+// before (their number, or with WEIGHT their weight) reaches a limit: `k`, or the part `p` of the
 // whole weight. The first token always stays.
 template <bool WEIGHT>
 __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {

@@ -378,7 +378,8 @@ def check_distill(lib, x, tv, ti, tgt, tau=1.0, alpha=1.0, scale=0.25, **kw):
     tol_row = t2 * (2 * rel + 6 * EPS * (2 * D + math.log(V) + 16))
     inf = ~np.isfinite(rr)
     assert np.array_equal(np.isinf(row), np.isinf(rr))
-    assert np.abs(row - rr)[~inf].max(initial=0.0) <= tol_row, (np.abs(row - rr)[~inf].max(), tol_row)
+    off = np.abs(row[~inf] - rr[~inf]).max(initial=0.0)
+    assert off <= tol_row, (off, tol_row)
     if inf.any():
         assert loss == rl
     else:
@@ -504,6 +505,37 @@ def test_distill_without_rows_writes_a_zero_loss(lib, cuda):
     abi.check(lib, lib.cngpt_cuda_distill(None, 10, 0, 10, None, None, 0, None, 1.0, 1.0, 1.0, ptr(loss), None, None, 0))
     abi.check(lib, lib.cngpt_cuda_check())
     assert float(loss[0]) == 0.0
+
+
+def test_largest_vocabularies(lib, cuda):
+    """The most that each entry point takes; one more is refused."""
+    x = logits(2, 262144, 30)
+    check_sample(lib, x, T=[0.8, 1.1], k=[40, 0], p=[0.9, 0.8], u=[0.3, 0.6])
+    x = logits(2, 400000, 31)
+    check_topk(lib, x, 70)
+    tv, ti, tgt = teacher(2, 400000, 40, 32)
+    check_distill(lib, x, tv, ti, tgt, 2.0, 0.5)
+    d = dev(x)
+    o, i = torch.empty(8, device="cuda"), torch.empty(8, dtype=torch.int32, device="cuda")
+    assert lib.cngpt_cuda_topk(ptr(d), 400001, 1, 400001, 2, ptr(o), ptr(i)) == abi.ERR_ARG
+    assert lib.cngpt_cuda_distill(ptr(d), 400001, 1, 400001, None, None, 0, ptr(i), 1.0, 0.0, 1.0, ptr(o), ptr(o), None,
+                                  0) == abi.ERR_ARG
+    assert lib.cngpt_cuda_sample(ptr(d), 262145, 1, 262145, None, None, None, None, ptr(o), ptr(i), None) == abi.ERR_ARG
+    lib.cngpt_cuda_clear_status()
+
+
+def test_distill_overlap_is_refused(lib, cuda):
+    d = torch.zeros(4, 64, device="cuda")
+    o, i = torch.zeros(8, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+
+    def call(out, ldd):
+        return lib.cngpt_cuda_distill(ptr(d), 64, 3, 60, None, None, 0, ptr(i), 1.0, 0.0, 1.0, ptr(o), ptr(o), out, ldd)
+    assert call(ptr(d) + 4, 64) == abi.ERR_ARG
+    assert call(ptr(d), 60) == abi.ERR_ARG
+    assert call(ptr(d) + 4 * 64, 64) == abi.ERR_ARG
+    assert call(ptr(torch.zeros(4, 64, device="cuda")), 59) == abi.ERR_ARG
+    assert call(ptr(d), 64) == abi.OK
+    lib.cngpt_cuda_clear_status()
 
 
 # ---------------------------------------------------------- streams, graphs
