@@ -5,25 +5,29 @@
 // inverted index), its weight exp((l - max) / T) in fixed point: 2^SH parts of the
 // largest weight, SH = 62 - log2(vocabulary), 50 at most, at least one part if it is not zero
 // in 64-bit floating point. Sums of such weights are exact whatever their order,
-// so atomics and any split of the row give the same token, and a border between
-// two tokens is off by at most V / 2^(SH + 1) parts, 1e-9 of the largest weight.
+// so atomics and any split of the row give the same token; a weight itself is right
+// to 1e-9, in fp32 and integer instructions (in fp64 ones it took twice as long).
 //
-// A cluster of blocks holds the row in shared memory. Both cuts of the ranking
+// A cluster of blocks holds the row in shared memory. Few tokens decide, and they
+// are found without ranking the others: a bar from the threads' maxima, which at
+// least k tokens (top-k up to 256) or some 300 (top-p) reach, or the bound of min-p.
+// With top-p one pass sums all weights and those from the bar on: do these hold top-p
+// of the whole, the border is among them. Up to 512 such tokens are ranked and drawn
+// from by one block. Otherwise both cuts of the ranking
 // (top-k: the first k keys; top-p: the keys before which less than p of the weight
 // lies) are thresholds on the key, found alike: a histogram of the counts or
-// weights over 1024 bins of max - l, whose prefix sums give the bin that the
+// weights over 1024 bins of the span in question, whose prefix sums give the bin that the
 // border falls into; the few hundred keys of that bin are then compared with one
 // another. Where a bin holds more than that (runs of equal logits, outliers that
-// stretch the bins), it is cut again by the bits of its keys until it does not. A
-// short top-k needs none of this: some 2 k tokens reach a bar that the threads'
-// maxima give, and one block draws among them.
+// stretch the bins), it is cut again by the bits of its keys until it does not.
 //
-// On B200: 1 x 50257 with top-k and top-p 14.3 us, 64 rows with min-p 11 us, 32 rows
-// with settings of their own 33 us, 256 rows by top-p alone 122 us (reading them:
-// 7.9 us). The last is bound by the shared-memory atomics of the weights (30
-// cycles a warp: half of the time) and by the exponentials; summing the weights in
-// limbs without returned values took twice as long, 26 KB stretches half more.
+// On B200: 1 x 50257 with top-k and top-p 12.8 us, 64 rows with min-p 11 us, 32 rows
+// with settings of their own 24 us, 256 rows by top-p alone 93 us (reading them:
+// 7.9 us; a histogram of every row 122 us). The last is bound by instruction issue:
+// some 60 a logit for its weight, and 15 % of the rows there have a nucleus of
+// thousands, whose histograms' atomics (30 cycles a warp) make them twice as long.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include <cooperative_groups.h>
@@ -44,23 +48,25 @@ constexpr int WARPS = NT / 32;
 constexpr int MAX_PARTS = 8;
 constexpr int SLICE_BYTES = 52 * 1024;  // of a row in a block's shared memory: three blocks an SM
 constexpr int BINS = 4 * NT;
-constexpr int TABLE = 64;    // entries 2^(j / 64) of the exponential
+constexpr int TABLE = 256;   // entries of the exponential, for 2^(-j / 256)
+constexpr double SHIFT = 0.51;  // the entries are those of j - SHIFT
 constexpr int BORDER = 512;  // keys that are compared with one another
+constexpr float ALL = NAN;   // as a high end: no logit is at or above it
 
 __device__ __forceinline__ u64 make_key(uint32_t rank, int i) { return ((u64)rank << 32) | (0xFFFFFFFFu - (uint32_t)i); }
 
-// 2^(j / TABLE) from the Taylor series of e^x, to the last bit or two
+// 2^31 2^((SHIFT - j) / TABLE) from the Taylor series of e^x
 struct Pow2 {
-    double v[TABLE];
+    uint32_t v[TABLE];
     constexpr Pow2() : v() {
         for (int j = 0; j < TABLE; ++j) {
-            const double x = 0.6931471805599453 * j / TABLE;
+            const double x = 0.6931471805599453 * (SHIFT - j) / TABLE;
             double term = 1.0, sum = 0.0;
             for (int n = 1; n < 30; ++n) {
                 sum += term;
                 term *= x / n;
             }
-            v[j] = sum;
+            v[j] = (uint32_t)(sum * 2147483648.0 + 0.5);
         }
     }
 };
@@ -80,18 +86,27 @@ struct Smem {
             u64 key[BORDER], measure[BORDER];  // the border's keys of all blocks
         };
     };
-    double table[TABLE];
+    uint32_t table[TABLE];
     u64 list[BORDER];  // this block's keys of the border
     Border mine;
     float max_of[MAX_PARTS], min_of[MAX_PARTS];
-    u64 sum_of[MAX_PARTS];
+    u64 total_of[MAX_PARTS], upper_of[MAX_PARTS], sum_of[MAX_PARTS];
     float bar_of[MAX_PARTS];
     int first_of[MAX_PARTS];
-    uint32_t fine_lo[NT], fine_hi[NT];
-    short list_of[BORDER];
+    union {
+        struct {
+            uint32_t fine_lo[NT], fine_hi[NT];
+        };
+        int index_of[BORDER];
+    };
+    union {
+        short list_of[BORDER];
+        int slot[BORDER];
+    };
+    __align__(16) uint32_t rank_of[BORDER];
     int few;
-    u64 warp[WARPS];
-    float fwarp[2][WARPS];
+    u64 warp[WARPS], upper[WARPS];
+    float fwarp[3][WARPS];
     float bar;
     __align__(16) float own[NT];
     int bin;
@@ -101,11 +116,11 @@ struct Smem {
 struct Row {
     const float *s;  // the block's stretch in shared memory
     int n, lo, per;  // its length, the index of its first token, tokens of a thread (odd: no bank conflicts)
-    float mx;
+    float mx, mf;    // the row's largest logit, and the largest finite one up to it
     double m, t, it; // maximum, temperature, 1 / temperature
-    double c;        // TABLE log2(e) / temperature
+    float ch, cl;    // TABLE log2(e) / temperature in two parts
     int sh;
-    const double *table;
+    const uint32_t *table;
     float cut_at;    // tokens above this logit stay, and of those at it
     int cut_index;   // the ones up to this index
 
@@ -121,10 +136,12 @@ struct Row {
             cut_index = 0x7FFFFFFF;
         }
     }
-    __device__ float gap(float x) const { return x == mx ? 0.0f : mx - x; }
     __device__ void cut(u64 key) {
-        cut_at = rank_value((uint32_t)(key >> 32));
-        cut_index = (int)(0xFFFFFFFFu - (uint32_t)key);
+        const float at = rank_value((uint32_t)(key >> 32));
+        const int i = (int)(0xFFFFFFFFu - (uint32_t)key);
+        if (!keeps(at, i)) return;  // below an earlier cut
+        cut_at = at;
+        cut_index = i;
     }
     // log of the weight; -inf for a finite logit beside a maximum of +inf
     __device__ double exponent(float x) const {
@@ -132,22 +149,26 @@ struct Row {
         const double d = (double)x - m;
         return isinf(d) ? d : d * it;
     }
-    // The weight in parts: 2^(z / 64) with z = k + f, |f| <= 1/2, as the table's
-    // 2^((k mod 64) / 64), its exponent raised by k / 64 + sh, times the Taylor
-    // series of 2^(f / 64) (the fifth power, 4e-14 of the weight, is left out).
-    // Adding 1.5 2^52 (2^52) leaves a rounded integer in the low bits.
+    // The weight of a token that stays, in parts, to 1e-9 of itself and rounded up: 2^(-z / 256) with z = (max - x) c in
+    // two floats (the difference's rounding error is exact, the product's an fma's).
+    // z = k + f - 0.51, 0 < f < 1.02, gives the table's entry for k mod 256 times
+    // 2^(-f / 256) = 1 - g as 32-bit fractions, moved down by k / 256; g from the
+    // Taylor series (the fourth power, 2e-12, is left out). Adding 1.5 2^23 to a
+    // float (2^23 to one above 0) leaves a rounded integer in its low bits.
     __device__ u64 weight(float x) const {
-        constexpr double B = 0.6931471805599453 / TABLE;
-        if (x == mx) return 1ull << sh;
-        const double z = ((double)x - m) * c;
-        if (z < -(double)(TABLE * (sh + 1))) return z < -745.0 / B ? 0 : 1;  // less than half a part
-        const double kd = z + 6755399441055744.0;
-        const int k = __double2loint(kd);
-        const double f = z - (kd - 6755399441055744.0);
-        const double q = fma(fma(fma(fma(B * B * B * B / 24, f, B * B * B / 6), f, B * B / 2), f, B), f, 1.0);
-        const double t = table[k & (TABLE - 1)];
-        const double w = __hiloint2double(__double2hiint(t) + ((k >> 6) + sh) * (1 << 20), __double2loint(t)) * q;
-        return max(1ull, (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull);
+        constexpr double B = 0.6931471805599453 / TABLE, F = 2147483648.0;
+        x = fminf(x, FLT_MAX);
+        const float d = __fsub_rn(mf, x), xr = __fsub_rn(mf, d), mr = __fadd_rn(d, xr);
+        const float dl = __fadd_rn(__fsub_rn(mf, mr), __fsub_rn(xr, x));
+        const float p = __fmul_rn(d, ch);
+        const float e = fmaf(dl, ch, fmaf(d, cl, fmaf(d, ch, -p)));
+        const float kd = __fadd_rn(p, 12582912.0f);
+        const uint32_t k = (uint32_t)__float_as_int(kd);  // 0x4B400000 + k
+        const float f = __fadd_rn(__fsub_rn(p, __fsub_rn(kd, 12582912.0f)), __fadd_rn(e, (float)SHIFT));
+        const float q = fmaf(fmaf((float)(F * B * B * B / 6), f, (float)(-F * B * B / 2)), f, (float)(F * B));
+        const uint32_t g = 2 * ((uint32_t)__float_as_int(fmaf(q, f, 8388608.0f)) - 0x4B000000u);
+        const u64 w = (u64)table[k & (TABLE - 1)] * (0xFFFFFFFFu - g);  // 2^63 parts of 1
+        return (w >> min(63u, k / TABLE - (uint32_t)(0x4B400000 / TABLE - 63 + sh))) + 1;
     }
 };
 
@@ -243,38 +264,47 @@ __device__ void gather(int n, int have, int parts, Smem &sm) {
 }
 
 // Raises r's cut to the border of the ranking at which the measure of the tokens
-// before (their number, or with WEIGHT their weight) reaches a limit: `k`, or the part `p` of the
-// whole weight. The first token always stays.
-template <bool WEIGHT>
-__device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
+// before (their number, or with WEIGHT their weight) reaches a limit below that of the
+// whole. It lies among the tokens from low_end up to but without high_end, and the
+// measure of those from high_end on is `above`.
+template <bool WEIGHT, class Each>
+__device__ void cut_ranking(Row &r, u64 limit, float low_end, float high_end, u64 above, Smem &sm, Each each) {
     auto cluster = coop::this_cluster();
     const int parts = (int)cluster.num_blocks(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int i0 = min(r.n, tid * r.per), i1 = min(r.n, i0 + r.per);
-    u64 above = 0, limit = k, lowest = 0, highest = 0;
+    u64 lowest = 0, highest = 0;
+    // bins over the span, at most 64 wide (an outlier would stretch them)
+    const float from = fminf(high_end, r.mx);
+    const float scale = low_end < from ? fminf((float)BINS / fminf(from - low_end, 64.0f), 1e30f) : 0.0f;
     int shift = 0;
     for (int level = 0;; ++level) {
         // bin of a token, the best ones first; -1: not (any more) in question
         auto bin_of = [&](float x, int i) {
-            if (level == 0) return r.keeps(x, i) ? (int)fminf(r.gap(x) * scale, (float)(BINS - 1)) : -1;
+            if (level == 0)
+                return x >= low_end && !(x >= high_end) && r.keeps(x, i)
+                           ? (int)fminf((x == from ? 0.0f : from - x) * scale, (float)(BINS - 1)) : -1;
             const u64 key = make_key(rank_key(x), i);
             return key >= lowest && key <= highest ? (int)((highest - key) >> shift) : -1;
         };
         *((uint4 *)sm.lo + tid) = make_uint4(0, 0, 0, 0);
         *((uint4 *)sm.hi + tid) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (int i = i0; i < i1; ++i) {
-            const float x = r.s[i];
-            const int b = bin_of(x, r.lo + i);
-            if (b < 0) continue;
-            if (!WEIGHT) {
-                atomicAdd(&sm.lo[b], 1u);
-            } else {
-                const u64 w = r.weight(x);
-                const uint32_t l = (uint32_t)w, old = atomicAdd(&sm.lo[b], l);
-                const uint32_t h = (uint32_t)(w >> 32) + (old + l < old ? 1u : 0u);  // with the carry
-                if (h) atomicAdd(&sm.hi[b], h);
+        each([&](const float(&x)[4], int i) {
+            int b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = bin_of(x[j], i + j);
+            if (max(max(b[0], b[1]), max(b[2], b[3])) < 0) return;
+            u64 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = WEIGHT ? r.weight(x[j]) : 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (b[j] < 0) continue;
+                const uint32_t l = (uint32_t)w[j], old = atomicAdd(&sm.lo[b[j]], l);
+                if (!WEIGHT) continue;
+                const uint32_t h = (uint32_t)(w[j] >> 32) + (old + l < old ? 1u : 0u);  // with the carry
+                if (h) atomicAdd(&sm.hi[b[j]], h);
             }
-        }
+        });
         cluster.sync();
         // thread t sums bins 4 t .. 4 t + 3 over the blocks; exclusive scan
         u64 c[4] = {}, s = 0;
@@ -302,12 +332,9 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
             if (w < warp) before += sm.warp[w];
             total += sm.warp[w];
         }
-        if (level == 0) {
-            if (WEIGHT) limit = max(1ull, (u64)ceil(p * (double)total));
-            if (total <= limit) {  // nothing to cut (the same in every block)
-                cluster.sync();    // the bins have been read
-                return;
-            }
+        if (!WEIGHT && level == 0 && total <= limit) {  // nothing to cut (the same in every block)
+            cluster.sync();                             // the bins have been read
+            return;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -322,15 +349,17 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
         above = sm.above;
         const int bin = sm.bin;
         u64 low = ~0ull, high = 0;
-        for (int i = i0; i < i1; ++i) {
-            const float x = r.s[i];
-            if (bin_of(x, r.lo + i) != bin) continue;
-            const u64 key = make_key(rank_key(x), r.lo + i);
-            const int at = atomicAdd(&sm.mine.count, 1);
-            if (at < BORDER) sm.list[at] = key;
-            low = min(low, key);
-            high = max(high, key);
-        }
+        each([&](const float(&x)[4], int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (bin_of(x[j], i + j) != bin) continue;
+                const u64 key = make_key(rank_key(x[j]), i + j);
+                const int at = atomicAdd(&sm.mine.count, 1);
+                if (at < BORDER) sm.list[at] = key;
+                low = min(low, key);
+                high = max(high, key);
+            }
+        });
         merge_span(low, high, sm);
         cluster.sync();  // also: the bins have been read
         // every warp: lane q asks block q, then warp q fetches block q's keys
@@ -365,91 +394,130 @@ __device__ void cut_ranking(Row &r, float scale, u64 k, double p, Smem &sm) {
     }
 }
 
-// The draw among sm.key[0, n), which hold the k first of the ranking, by one block.
+// The draw by one block among sm.key[0, n), which hold the first k of the ranking;
+// those stay before which less than `limit` of the weight lies (0: less than the
+// part p of theirs).
 template <class Put>
-__device__ void draw_brief(Row &r, int n, int k, float p, float min_p, float u, Smem &sm, Put put) {
+__device__ void draw_brief(Row &r, int n, int k, u64 limit, float p, float min_p, float u, Smem &sm, Put put) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto logit = [&](int e) { return rank_value((uint32_t)(sm.key[e] >> 32)); };
-    auto index = [&](int e) { return (int)(0xFFFFFFFFu - (uint32_t)sm.key[e]); };
-    auto span = [&](u64 &lowest, u64 &highest) {
-        if (tid == 0) sm.mine = {0, ~0ull, 0};
-        __syncthreads();
-        lowest = ~0ull;
-        highest = 0;
-        for (int e = tid; e < n; e += NT) {
-            lowest = min(lowest, sm.key[e]);
-            highest = max(highest, sm.key[e]);
-        }
-        merge_span(lowest, highest, sm);
-        __syncthreads();
-        lowest = sm.mine.lowest;
-        highest = sm.mine.highest;
-    };
-    auto sum = [&](u64 v) {
-        v = warp_scan(v, lane);
-        __syncthreads();
-        if (lane == 31) sm.warp[warp] = v;
-        __syncthreads();
-        v = 0;
-        for (int w = 0; w < WARPS; ++w) v += sm.warp[w];
-        return v;
-    };
-    u64 lowest, highest;
-    span(lowest, highest);
-    if (n > k) r.cut(border_cut(n, lowest, highest, 0, (u64)k, false, sm));
-    u64 s = 0;
-    for (int e = tid; e < n; e += NT) s += sm.measure[e] = r.keeps(logit(e), index(e)) ? r.weight(logit(e)) : 0;
-    u64 total = sum(s);
-    if (p < 1.0f) {
-        const u64 limit = max(1ull, (u64)ceil((double)p * (double)total));
-        if (limit < total) r.cut(border_cut(n, lowest, highest, 0, limit, true, sm));
+    constexpr int PER = BORDER / NT;
+    auto logit = [&](int e) { return rank_value((uint32_t)(sm.list[e] >> 32)); };
+    auto index = [&](int e) { return (int)(0xFFFFFFFFu - (uint32_t)sm.list[e]); };
+    // The ranking: a key's place is the number of larger logits, those with as many
+    // (equal ones) are told apart by their indices.
+    for (int e = tid; e < BORDER; e += NT) {
+        sm.rank_of[e] = e < n ? (uint32_t)(sm.key[e] >> 32) : 0;
+        sm.slot[e] = 0;
     }
-    r.least(min_p);
-    // those that stay, close together: index and weight
-    int *at = (int *)sm.fine_lo;
-    u64 *weight = sm.list;
-    if (tid == 0) sm.few = 0;
-    s = 0;
-    for (int e = tid; e < n; e += NT)
-        if (sm.measure[e] && r.keeps(logit(e), index(e))) s += sm.measure[e];
-    total = sum(s);
-    for (int e = tid; e < n; e += NT)
-        if (sm.measure[e] && r.keeps(logit(e), index(e))) {
-            const int j = atomicAdd(&sm.few, 1);  // at most k <= NT
-            at[j] = index(e);
-            weight[j] = sm.measure[e];
-            sm.list_of[j] = (short)e;
-        }
     __syncthreads();
-    n = sm.few;
+    int place[PER] = {};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = tid + j * NT;
+        if (e >= n) break;
+        const uint32_t mine = sm.rank_of[e];
+#pragma unroll 4
+        for (int q = 0; q < n; q += 4) {
+            const uint4 o = *(const uint4 *)(sm.rank_of + q);
+            place[j] += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+        }
+        atomicAdd(&sm.slot[place[j]], 1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = tid + j * NT;
+        if (e >= n) break;
+        const u64 key = sm.key[e];
+        if (sm.slot[place[j]] > 1)
+            for (int q = 0; q < n; ++q) place[j] += sm.key[q] > key && sm.key[q] >> 32 == key >> 32;
+        sm.list[place[j]] = key;
+        const float x = rank_value((uint32_t)(key >> 32));
+        sm.measure[place[j]] = r.keeps(x, (int)(0xFFFFFFFFu - (uint32_t)key)) ? r.weight(x) : 0;
+    }
+    __syncthreads();
+    // its running sums, two tokens a thread; those that stay come first
+    u64 w[PER], s = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) s += w[j] = PER * tid + j < min(n, k) ? sm.measure[PER * tid + j] : 0;
+    u64 before = warp_scan(s, lane), total = 0;
+    if (lane == 31) sm.warp[warp] = before;
+    __syncthreads();
+    before -= s;
+    for (int q = 0; q < WARPS; ++q) {
+        if (q < warp) before += sm.warp[q];
+        total += sm.warp[q];
+    }
+    if (!limit) limit = p < 1.0f ? max(1ull, (u64)ceil((double)p * (double)total)) : total;
+    r.least(min_p);
+    bool stay[PER];
+    u64 upto[PER];
+    int left = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = PER * tid + j;
+        stay[j] = w[j] && before < limit && r.keeps(logit(e), index(e));
+        upto[j] = before += w[j];
+        left += __syncthreads_count(stay[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int e = PER * tid + j;
+        if (stay[j]) sm.index_of[e] = index(e);
+        if (e == left - 1) sm.above = upto[j];
+    }
+    __syncthreads();
+    total = sm.above;
+    const int *at = sm.index_of;
+    const u64 *weight = sm.measure;
     const u64 target = u < 1.0f ? min(total - 1, (u64)fmax(0.0, (double)u * (double)total)) : total - 1;
     const double whole = ldexp((double)total, -r.sh);
     if (target == 0 && u > 0.0f) {  // below one part: the weights as they are, see sample_kernel
         if (tid != 0) return;
         double c = 0.0;
-        for (int last = -1, left = n;; --left) {
+        for (int last = -1, more = left;; --more) {
             int e = -1;  // the next one in index order
-            for (int j = 0; j < n; ++j)
+            for (int j = 0; j < left; ++j)
                 if (at[j] > last && (e < 0 || at[j] < at[e])) e = j;
             last = at[e];
-            const double y = r.exponent(logit(sm.list_of[e]));
+            const double y = r.exponent(logit(e));
             c += exp(y);
-            if (c > (double)u * whole || left == 1) {
+            if (c > (double)u * whole || more == 1) {
                 put(last, (float)(y - log(whole)));
                 return;
             }
         }
     }
-    for (int e = tid; e < n; e += NT) {
-        u64 before = 0;
+    if (left <= NT / 2) {  // each against the others
+        if (tid >= left) return;
+        u64 lower = 0;
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) before += at[j] < at[e] ? weight[j] : 0;
-        if (before <= target && before + weight[e] > target)
-            put(at[e], (float)(r.exponent(logit(sm.list_of[e])) - log(whole)));
+        for (int j = 0; j < left; ++j) lower += at[j] < at[tid] ? weight[j] : 0;
+        if (lower <= target && lower + weight[tid] > target)
+            put(at[tid], (float)(r.exponent(logit(tid)) - log(whole)));
+        return;
+    }
+    // The first in index order whose sum exceeds the target: with the index as the
+    // key's upper half the lowest before which it does not.
+    if (tid == 0) sm.mine = {0, ~0ull, 0};
+    __syncthreads();
+    u64 lowest = ~0ull, highest = 0;
+    for (int e = tid; e < left; e += NT) {
+        const u64 key = sm.list[e] << 32 | sm.list[e] >> 32;
+        sm.key[e] = key;
+        lowest = min(lowest, key);
+        highest = max(highest, key);
+    }
+    merge_span(lowest, highest, sm);
+    __syncthreads();
+    const u64 drawn = border_cut(left, sm.mine.lowest, sm.mine.highest, 0, target + 1, true, sm);
+    if (tid == 0) {
+        const float v = rank_value((uint32_t)drawn);
+        put((int)(0xFFFFFFFFu - (uint32_t)(drawn >> 32)), (float)(r.exponent(v) - log(whole)));
     }
 }
 
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, 3)
 sample_kernel(SampleRows a, int stretch, int sh) {
     extern __shared__ float4 slice4[];
     __shared__ __align__(16) Smem sm;
@@ -476,10 +544,12 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     if (odd >= 0)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slice + pad + odd)), "l"(x + odd) : "memory");
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const float T = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
+    float T = a.temperature ? a.temperature[row] : 1.0f;
+    if (T > 0.0f) T = fminf(fmaxf(T, 0x1p-100f), 0x1p100f);  // the exponential's range
+    const float p = a.top_p ? a.top_p[row] : 1.0f;
     const float min_p = a.min_p ? a.min_p[row] : 0.0f, u = a.u[at];
     const int k = a.top_k ? a.top_k[row] : 0;
-    if (tid < TABLE) sm.table[tid] = pow2_table.v[tid];
+    sm.table[tid] = pow2_table.v[tid];
     auto put = [&](int token, float logprob) {
         a.tokens[at] = token;
         if (a.next) a.next[row] = max(token, 0);
@@ -508,9 +578,24 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     const float own = mx;  // of this thread
     mx = warp_max(mx);
     mn = -warp_max(-mn);
+    // a bar for top-p that some 300 tokens reach: the mean over the row's warps of the
+    // one of the lanes' maxima that 256 of the row's (22 of a lone block's warp) reach
+    const bool nucleus = !brief && T > 0.0f && p > 0.0f && p < 1.0f;
+    float reach = -INFINITY;
+    if (nucleus && a.V > BORDER) {
+        int rank = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            const float v = __shfl_sync(0xffffffffu, own, j);
+            rank += v > own || (v == own && j < lane);
+        }
+        const int at = 31 - __clz(__ballot_sync(0xffffffffu, rank == min(22, 32 / parts) - 1));
+        reach = __shfl_sync(0xffffffffu, own, at);
+    }
     if (lane == 0) {
         sm.fwarp[0][warp] = mx;
         sm.fwarp[1][warp] = mn;
+        sm.fwarp[2][warp] = reach;
         if (warp == 0) sm.mine = {0, ~0ull, 0};
     }
     sm.own[tid] = own;
@@ -518,6 +603,16 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     for (int w = 0; w < WARPS; ++w) {
         mx = fmaxf(mx, sm.fwarp[0][w]);
         mn = fminf(mn, sm.fwarp[1][w]);
+    }
+    if (nucleus) {
+        float s = 0.0f;
+        int n = 0;
+        for (int w = 0; w < WARPS; ++w)
+            if (sm.fwarp[2][w] > -INFINITY) {
+                s += sm.fwarp[2][w];
+                ++n;
+            }
+        reach = n ? s / n : -INFINITY;
     }
     if (brief) {
         int rank = 0;
@@ -530,7 +625,7 @@ sample_kernel(SampleRows a, int stretch, int sh) {
         if (rank == (k + parts - 1) / parts - 1) sm.bar = own;  // exactly one thread
         __syncthreads();
     }
-    float bar = brief ? sm.bar : -INFINITY;
+    float bar = brief ? sm.bar : reach;
     cluster.barrier_wait();
     if (tid < parts) {
         *cluster.map_shared_rank(&sm.max_of[part], tid) = mx;
@@ -542,6 +637,16 @@ sample_kernel(SampleRows a, int stretch, int sh) {
         mx = fmaxf(mx, sm.max_of[q]);
         mn = fminf(mn, sm.min_of[q]);
         bar = fminf(bar, sm.bar_of[q]);
+    }
+    if (nucleus) {
+        float s = 0.0f;
+        int n = 0;
+        for (int q = 0; q < parts; ++q)
+            if (sm.bar_of[q] > -INFINITY) {
+                s += sm.bar_of[q];
+                ++n;
+            }
+        bar = n ? s / n : -INFINITY;
     }
     if (mx == -INFINITY) {  // the same in every block, as all that follows
         if (part == 0 && tid == 0) put(-1, -INFINITY);
@@ -571,46 +676,143 @@ sample_kernel(SampleRows a, int stretch, int sh) {
     r.m = (double)mx;
     r.t = (double)T;
     r.it = 1.0 / r.t;
-    r.c = TABLE * 1.4426950408889634 * r.it;
-    r.cut_at = -INFINITY;
+    const double factor = TABLE * 1.4426950408889634 * r.it;
+    r.ch = (float)factor;
+    r.cl = (float)(factor - (double)r.ch);
+    r.mf = fminf(mx, FLT_MAX);
+    // nothing stays beside +inf, nor what has no weight in 64-bit floating point
+    r.cut_at = fminf(__double2float_rd(r.m - 745.0 * r.t), nextafterf(mx, -INFINITY));
+    if (mx == INFINITY) r.cut_at = FLT_MAX;
     r.cut_index = -1;
-    if (bar > -INFINITY) {
-        // A short top-k: the tokens that reach the bar, some 2 k, decide alone.
-        if (own >= bar) {
-            auto check = [&](float v, int i) {
-                if (v >= bar) {
-                    const int e = atomicAdd(&sm.mine.count, 1);
-                    if (e < BORDER) sm.list[e] = make_key(rank_key(v), r.lo + i);
-                }
-            };
-            if (odd >= 0) check(r.s[odd], odd);
-#pragma unroll 2
-            for (int q = tid; q < quads; q += NT) {
-                const float4 v = s4[q];
-                if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bar) {
-                    check(v.x, head + 4 * q);
-                    check(v.y, head + 4 * q + 1);
-                    check(v.z, head + 4 * q + 2);
-                    check(v.w, head + 4 * q + 3);
-                }
+    // the stretch's logits in no order, four at a time (NaN: none), whose weights
+    // have no need to wait for one another
+    auto each = [&](auto &&f) {
+        for (int q = tid - NT; q < quads; q += NT) {
+            float v[4] = {NAN, NAN, NAN, NAN};
+            if (q >= 0) {
+                const float4 w = s4[q];
+                v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+                f(v, r.lo + head + 4 * q);
+            } else if (odd >= 0) {
+                v[0] = r.s[odd];
+                f(v, r.lo + odd);
             }
         }
+    };
+    // the tokens that reach a bar, to the list
+    auto collect = [&](float v, int i) {
+        const int e = atomicAdd(&sm.mine.count, 1);
+        if (e < BORDER) sm.list[e] = make_key(rank_key(v), i);
+    };
+    // in all blocks, after the next cluster.sync(): their number; and block 0 draws among them
+    auto listed = [&](int &have) {
+        have = lane < parts ? cluster.map_shared_rank(&sm.mine, lane)->count : 0;
+        return __reduce_add_sync(0xffffffffu, have);
+    };
+    auto draw = [&](int n, int have, int first, u64 limit) {
+        if (part == 0) gather(n, have, parts, sm);
+        cluster.sync();  // the others' keys have been read
+        if (part == 0) draw_brief(r, n, first, limit, p, min_p, u, sm, put);
+    };
+    if (brief && bar > -INFINITY) {
+        // A short top-k: the tokens that reach the bar, some 2 k, decide alone.
+        if (own >= bar)
+            each([&](const float(&v)[4], int i) {
+                if (!(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= bar)) return;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (v[j] >= bar) collect(v[j], i + j);
+            });
         cluster.sync();
-        const int have = lane < parts ? cluster.map_shared_rank(&sm.mine, lane)->count : 0;
-        const int n = __reduce_add_sync(0xffffffffu, have);
+        int have;
+        const int n = listed(have);
         if (n <= BORDER) {
-            if (part == 0) gather(n, have, parts, sm);
-            cluster.sync();  // the others' keys have been read
-            if (part == 0) draw_brief(r, n, k, p, min_p, u, sm, put);
+            draw(n, have, k, 0);
             return;
         }
         // too many equal logits: the general way
     }
-    // bins over the row's span, at most 64 wide (an outlier would stretch them)
-    const float scale = mn < mx ? fminf((float)BINS / fminf(mx - mn, 64.0f), 1e30f) : 0.0f;
-    if (k > 0 && k < a.V) cut_ranking<false>(r, scale, (u64)k, 0.0, sm);
-    if (p < 1.0f) cut_ranking<true>(r, scale, 0, (double)p, sm);
-    r.least(min_p);
+    if (k > 0 && k < a.V) {
+        cut_ranking<false>(r, (u64)k, mn, ALL, 0, sm, each);
+        cluster.sync();  // the blocks' lists have been read
+    }
+    if (tid == 0) sm.mine = {0, ~0ull, 0};
+    __syncthreads();
+    if (p < 1.0f) {
+        // the whole weight, and the tokens that reach the bar with theirs
+        u64 s = 0, upper = 0;
+        each([&](const float(&v)[4], int i) {
+            u64 kept[4];
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const u64 w = r.weight(v[e]);
+                kept[e] = r.keeps(v[e], i + e) ? w : 0;
+                s += kept[e];
+                any |= v[e] >= bar;
+            }
+            if (!any) return;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v[e] >= bar && kept[e]) {
+                    upper += kept[e];
+                    collect(v[e], i + e);
+                }
+        });
+        s = warp_scan(s, lane);
+        upper = warp_scan(upper, lane);
+        if (lane == 31) {
+            sm.warp[warp] = s;
+            sm.upper[warp] = upper;
+        }
+        __syncthreads();
+        if (tid < 2 * parts) {
+            const u64 *of = tid < parts ? sm.warp : sm.upper;
+            u64 v = 0;
+            for (int w = 0; w < WARPS; ++w) v += of[w];
+            *cluster.map_shared_rank(&(tid < parts ? sm.total_of : sm.upper_of)[part], tid % parts) = v;
+        }
+        cluster.sync();
+        u64 whole = 0;
+        upper = 0;
+        for (int q = 0; q < parts; ++q) {
+            whole += sm.total_of[q];
+            upper += sm.upper_of[q];
+        }
+        const u64 limit = max(1ull, (u64)ceil((double)p * (double)whole));
+        int have;
+        const int n = listed(have);
+        if (n <= BORDER && limit < whole && limit <= upper) {
+            draw(n, have, n, limit);
+            return;
+        }
+        if (limit < whole) {
+            // A wide nucleus. Its border is not below a floor: V tokens under it would weigh
+            // less than what lies behind the border; two parts (for the rounding) less than
+            // an equal share, and 1e-8 of it for the exponential's error.
+            const double share = ldexp((double)(whole - limit) / a.V - 2.0, -sh) * (1.0 - 1e-8);
+            const float floor = share > 0.0 ? fminf(mx, __double2float_rd(r.m + r.t * log(share))) : -INFINITY;
+            if (limit <= upper)
+                cut_ranking<true>(r, limit, fmaxf(bar, mn), ALL, 0, sm, each);
+            else
+                cut_ranking<true>(r, limit, fmaxf(floor, mn), bar, upper, sm, each);
+        }
+        r.least(min_p);
+    } else if (min_p > 0.0f) {
+        r.least(min_p);
+        each([&](const float(&v)[4], int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (r.keeps(v[e], i + e)) collect(v[e], i + e);
+        });
+        cluster.sync();
+        int have;
+        const int n = listed(have);
+        if (n <= BORDER) {
+            draw(n, have, n, 0);
+            return;
+        }
+    }
 
     // cumulative weights in index order: threads, warps, blocks
     auto drawn = [&](int i) -> u64 {
@@ -618,10 +820,20 @@ sample_kernel(SampleRows a, int stretch, int sh) {
         return r.keeps(v, r.lo + i) ? r.weight(v) : 0;
     };
     u64 s = 0;
-    for (int j = i0; j < i1; j += 32) {  // which of 32 stay, then the weights of those alone
-        uint32_t stay = 0;
-        for (int i = j; i < min(i1, j + 32); ++i) stay |= r.keeps(r.s[i], r.lo + i) ? 1u << (i - j) : 0u;
-        for (; stay; stay &= stay - 1) s += r.weight(r.s[j + __ffs(stay) - 1]);
+    for (int i = i0; i < i1; i += 4) {  // four that need not wait for one another
+        float v[4];
+        bool stay[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = i + e < i1 ? r.s[i + e] : NAN;
+            stay[e] = r.keeps(v[e], r.lo + i + e);
+        }
+        if (!(stay[0] || stay[1] || stay[2] || stay[3])) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u64 w = r.weight(v[e]);
+            s += stay[e] ? w : 0;
+        }
     }
     const u64 inc = warp_scan(s, lane);
     if (lane == 31) sm.warp[warp] = inc;
@@ -705,7 +917,7 @@ int sample_rows(const SampleRows &a, cudaStream_t s) {
     // more while there are rows for half the SMs at most.
     int parts = 1;
     while (parts < MAX_PARTS && ((long)a.V * 4 > (long)parts * SLICE_BYTES ||
-                                 ((long)a.rows * parts * 2 <= num_sms() && a.V >= parts * 2048)))
+                                 ((long)a.rows * parts <= num_sms() && a.V >= parts * 2048)))
         parts *= 2;
     if ((long)a.rows * parts > 0x7FFFFFFFL) {
         set_last_error(ERR_ARG, "sample: %d rows are too many", a.rows);

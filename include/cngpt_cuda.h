@@ -124,9 +124,10 @@ int cngpt_cuda_layernorm_bwd_noalloc(const float *dout, const float *x, const fl
  * kept tokens exceeds u times their sum. temperature <= 0 (or NaN) takes the
  * first of the ranking. Logits that are -inf or NaN are never drawn; +inf
  * logits share the draw equally. A row in which nothing can be drawn gives
- * token -1 and logprob -inf. Weights and sums are held in 64 bits, so the token
- * does not depend on rounding unless u lies within about 1e-9 of a border, and
- * the same inputs always give the same token.
+ * token -1 and logprob -inf. A temperature below 2^-100 counts as 2^-100, one
+ * above 2^100 as 2^100. Weights are right to about 1e-9 and their sums exact in 64
+ * bits, so the token does not depend on rounding unless u or top_p lies within
+ * about 1e-9 of a border, and the same inputs always give the same token.
  * logprob (may be NULL): the log of the probability with which the token was
  * drawn among the kept ones (0 for a greedy row).
  * 1 <= vocab <= 262144. */

@@ -89,7 +89,7 @@ def check_sample(lib, x, T=None, k=None, p=None, mp=None, u=None, ld=None, shift
         t, l = ref_sample(x[r], one(T, r, 1.0), int(one(k, r, 0)), one(p, r, 1.0), one(mp, r, 0.0), float(u[r]))
         assert got[r] == t, (r, got[r], t)
         # the log is rounded once; the weights' sum is held to about 1e-9
-        assert glp[r] == l or abs(glp[r] - l) <= EPS * abs(l) + 1e-8, (r, glp[r], l)
+        assert glp[r] == l or abs(float(glp[r]) - l) <= EPS * abs(l) + 1e-8, (r, glp[r], l)  # in 64 bits
     return got[:rows]
 
 
@@ -201,6 +201,28 @@ def test_sample_flat_rows_keep_most_of_the_vocabulary(lib, cuda):
     check_sample(lib, x, p=g.uniform(0.3, 0.99, 12), u=g.random(12))
     check_sample(lib, x, k=g.integers(10000, 50000, 12), u=g.random(12))
     check_sample(lib, x, k=g.integers(10000, 50000, 12), p=g.uniform(0.3, 0.99, 12), u=g.random(12))
+
+
+@pytest.mark.parametrize("V", [513, 2000, 20011, 50257, 262144])
+@pytest.mark.parametrize("rows", [1, 24])
+def test_sample_nuclei_from_one_token_to_all(lib, cuda, rows, V):
+    """top-p over rows whose nucleus is a few tokens, some hundreds, thousands, or
+    cut out of a run of equal logits, with the whole mass in any part of the row."""
+    g = np.random.default_rng(V + rows)
+    base = logits(8, V, V, spread=1.0)
+    base[1] *= 8.0                                   # a few tokens
+    base[2] = np.float32(0.01) * base[2]             # nearly flat
+    base[3, g.permutation(V)[:600]] = 9.0            # a run of equal ones around the border
+    base[4, : V - 400] = -INF                        # all in the last stretch
+    base[5, g.random(V) < 0.97] = -INF
+    base[6] = np.where(g.random(V) < 0.5, np.float32(1.0), np.float32(0.0))  # two values
+    base[7, 5] = 60.0                                # one token outweighs the others
+    x = base[np.arange(rows) % 8] if rows > 1 else base[3:4]
+    p = g.choice([0.05, 0.3, 0.6, 0.9, 0.97, 0.9999], rows)
+    check_sample(lib, x, T=g.choice([0.01, 0.4, 1.0, 30.0], rows), p=p, u=g.random(rows))
+    check_sample(lib, x, T=g.choice([0.7, 1.0], rows), p=p, mp=g.uniform(0.0, 0.3, rows), u=g.random(rows))
+    check_sample(lib, x, k=np.full(rows, min(V, 700)), p=p, u=g.random(rows))
+    check_sample(lib, x, k=np.full(rows, 200), p=p, mp=np.full(rows, 0.01), u=g.random(rows))
 
 
 def test_sample_without_logprob_and_repeatable(lib, cuda):
