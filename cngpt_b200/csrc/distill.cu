@@ -51,11 +51,14 @@ struct Stats {
 
 __device__ __forceinline__ float scaled_max(float m, float c) { return m == -INFINITY ? 0.0f : __fmul_rn(m, c); }
 
-// the sums of `s` relative to the maximum m >= s.m
+// the sums of `s` relative to the maximum m >= s.m; those of a part of -inf alone
+// stay what they are (0, or NaN), whatever R(m) is
 template <bool BOTH>
 __device__ __forceinline__ void raise(Stats &s, float m, float ct) {
-    s.st *= ex2(scaled_max(s.m, ct) - scaled_max(m, ct));
-    if (BOTH) s.s1 *= ex2(scaled_max(s.m, LOG2E) - scaled_max(m, LOG2E));
+    if (s.m > -INFINITY) {
+        s.st *= ex2(scaled_max(s.m, ct) - scaled_max(m, ct));
+        if (BOTH) s.s1 *= ex2(scaled_max(s.m, LOG2E) - scaled_max(m, LOG2E));
+    }
     s.m = m;
 }
 

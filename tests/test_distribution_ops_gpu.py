@@ -442,6 +442,24 @@ def test_distill_strides_and_alignment(lib, cuda, ld, shift, ldd):
     check_distill(lib, x, tv, ti, tgt, 2.0, 0.6, ld=ld, shift=shift, inplace=True)
 
 
+@pytest.mark.parametrize("V", [97, 4099, 50257])
+@pytest.mark.parametrize("tau,alpha", [(1.0, 0.5), (2.0, 1.0)])
+def test_distill_far_below_zero_beside_masked_stretches(lib, cuda, V, tau, alpha):
+    """Logits far below 0 next to warps and blocks that hold -inf alone: a part
+    without weight must not be scaled by 2^(0 - R)."""
+    tv, ti, tgt = teacher(5, V, 8, V)
+    x = logits(5, V, V) - np.float32(400.0)
+    first = (V + 1) // 2
+    x[0, :first], x[1, first:], x[2, : V - 3] = -INF, -INF, -INF
+    x[3, np.arange(V) % 1024 < min(128, V // 2)] = -INF  # of some warps every group of four
+    for r in range(5):
+        live = np.flatnonzero(x[r] > -INF)
+        ti[r] = live[np.arange(8) % live.size]
+        tgt[r] = live[-1]
+    check_distill(lib, x, tv, ti, tgt, tau, alpha)
+    check_distill(lib, x, tv, ti, tgt, tau, alpha, grad=False)
+
+
 @pytest.mark.parametrize("V", [97, 50257])
 def test_distill_padding_duplicates_and_empty_rows(lib, cuda, V):
     g = np.random.default_rng(V)
