@@ -10,12 +10,17 @@
 // gradient), so a cluster of blocks keeps the row in its shared memory between
 // the pass that forms the sums and the pass that writes.
 //
-// On B200, 8192 x 50257 with both softmaxes and the gradient: 0.755 ms (4.4 TB/s, 67 %
-// of the copy rate); the loss of 1024 rows alone: 60 us (3.4 TB/s). What is left is the
+// The list's dependent loads, its softmax and the second writing of its entries are
+// one warp's; eight others look after the stretch and wait for it only at the end
+// (with the list's warp among them they waited twice: 0.76 ms where it is 0.675).
+//
+// On B200, 8192 x 50257 with both softmaxes and the gradient: 0.675 ms (4.9 TB/s, 75 %
+// of the copy rate); the loss of 1024 rows alone: 56.6 us (3.6 TB/s). What is left is the
 // latency of a row's phases (loads, two block barriers, one cluster barrier), which
 // four blocks an SM do not hide; the exponentials take half of the special-function
-// units' time. Smaller and larger blocks and stretches took 0.756 to 1.24 ms,
-// clusters that prefetch their next row 2.0 ms (the list's loads delay every row).
+// units' time. Two to seven more warps took 0.68 to 1.09 ms, shorter stretches 1.06,
+// sums of chunks while the next ones arrive 8 % more, clusters that prefetch their
+// next row three times as long.
 #include <algorithm>
 #include <cmath>
 
@@ -31,7 +36,8 @@ namespace coop = cooperative_groups;
 
 #define LAUNCH_CHECK() do { ++g_launch_count; CG_CUDA(cudaGetLastError()); } while (0)
 
-constexpr int NT = 256;
+constexpr int COPY = 256;      // threads of the stretch, behind
+constexpr int NT = 32 + COPY;  // the list's warp
 constexpr int MAX_PARTS = 8;
 constexpr int SLICE_BYTES = 52 * 1024;  // of a row in a block's shared memory: four blocks an SM
 constexpr float LOG2E = 1.4426950408889634f;
@@ -78,13 +84,14 @@ struct DistillArgs {
 
 // Cluster of 1 to 8 blocks per row, a stretch of it each. BOTH: the hard part's
 // softmax (temperature 1) is needed beside the list's. Warp 0 looks after the
-// list; every thread reads from shared memory only what it copied there itself.
+// list; until the first barrier the others read from shared memory only what they
+// copied there themselves.
 template <bool GRAD, bool BOTH>
 __global__ void __launch_bounds__(NT)
 distill_kernel(DistillArgs a) {
     extern __shared__ float4 slice4[];  // [stretch + 8], then the list: sp, sx, si [k]
     __shared__ Stats sw[NT / 32], sc[MAX_PARTS];
-    __shared__ int twice, listed;
+    __shared__ int soft_list, twice, listed;
     float *slice = (float *)slice4, *sp = slice + a.stretch + 8, *sx = sp + a.k;
     int *si = (int *)(sx + a.k);
     auto cluster = coop::this_cluster();
@@ -98,9 +105,10 @@ distill_kernel(DistillArgs a) {
     // elements before the first 16-byte boundary, whole groups of four, the rest;
     // element i of the stretch is kept at slice[pad + i], groups at float4s
     const int head = min(n, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (n - head) / 4, pad = (4 - head) & 3;
-    const int odd = tid < head ? tid : tid < n - 4 * quads ? tid + 4 * quads : -1;  // this thread's of those at both ends
+    const int at = tid - 32;  // among the threads of the stretch
+    const int odd = at < 0 ? -1 : at < head ? at : at < n - 4 * quads ? at + 4 * quads : -1;  // this thread's of those at both ends
     float4 *s4 = (float4 *)(slice + pad + head);
-    for (int q = tid; q < quads; q += NT)
+    for (int q = at; at >= 0 && q < quads; q += COPY)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s4 + q)), "l"(x + head + 4 * q) : "memory");
     if (odd >= 0)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slice + pad + odd)), "l"(x + odd) : "memory");
@@ -127,7 +135,7 @@ distill_kernel(DistillArgs a) {
 
     // statistics of the thread, the warp, the block and the row, in a fixed order
     Stats s{-INFINITY, 0.0f, 0.0f};
-    for (int q = tid; q < quads; q += NT) {
+    for (int q = at; at >= 0 && q < quads; q += COPY) {
         const float4 v = s4[q];
         s.m = fmaxf(s.m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
@@ -139,7 +147,7 @@ distill_kernel(DistillArgs a) {
             if (BOTH) s.s1 += ex2(fmaf(v, LOG2E, -r1));
         };
 #pragma unroll 2
-        for (int q = tid; q < quads; q += NT) {
+        for (int q = at; at >= 0 && q < quads; q += COPY) {
             const float4 v = s4[q];
             add(v.x);
             add(v.y);
@@ -152,6 +160,7 @@ distill_kernel(DistillArgs a) {
         if (BOTH) s.s1 = warp_sum(s.s1);
     }
     if (lane == 0) sw[warp] = s;
+    if (tid == 0) soft_list = lm > -INFINITY;
     __syncthreads();
     auto join = [&](const Stats *v, int count) {
         float m = v[0].m;
@@ -176,10 +185,7 @@ distill_kernel(DistillArgs a) {
     }
     const float rt = scaled_max(s.m, ct), r1 = scaled_max(s.m, LOG2E);
     const bool live = !(s.m == -INFINITY && s.st == 0.0f);
-    lm = __shfl_sync(0xffffffffu, lm, 0);
-    if (tid == 0) twice = live && lm > -INFINITY;  // hands "soft" to the block until it counts company
-    bool soft = live && lm > -INFINITY;            // so far right in warp 0 alone
-    const bool hard = live && has_tgt;
+    const bool soft = live && soft_list, hard = live && has_tgt;
     if (warp == 0) {
         float loss = 0.0f;
         if (soft) {
@@ -200,9 +206,6 @@ distill_kernel(DistillArgs a) {
         if (part == 0 && lane == 0) a.row_loss[row] = loss;
     }
     if (!GRAD) return;
-    __syncthreads();
-    soft = twice;
-
     float *dr = a.dlogits + row * a.ldd, *d = dr + lo;
     const float ot = a.scale * a.alpha * a.tau, o1 = a.scale * (1.0f - a.alpha);
     const float gt = soft ? ot / s.st : 0.0f, g1 = BOTH && hard ? o1 / s.s1 : 0.0f;
@@ -213,14 +216,14 @@ distill_kernel(DistillArgs a) {
         return none ? 0.0f : g;
     };
     if (odd >= 0) d[odd] = grad(slice[pad + odd]);
-    if (((uintptr_t)(d + head) & 15) == 0) {  // the groups of x are groups of d too
+    if (((uintptr_t)(d + head) & 15) == 0 && warp > 0) {  // the groups of x are groups of d too
 #pragma unroll 2
-        for (int q = tid; q < quads; q += NT) {
+        for (int q = at; q < quads; q += COPY) {
             const float4 v = s4[q];
             __stcs((float4 *)(d + head) + q, make_float4(grad(v.x), grad(v.y), grad(v.z), grad(v.w)));
         }
-    } else {  // another alignment: element by element, from the whole block's copies
-        for (int i = head + tid; i < head + 4 * quads; i += NT) d[i] = grad(slice[pad + i]);
+    } else if (warp > 0) {  // another alignment: element by element, from the whole block's copies
+        for (int i = head + at; i < head + 4 * quads; i += COPY) d[i] = grad(slice[pad + i]);
     }
     if (none) return;
     __syncthreads();
