@@ -11,6 +11,7 @@
 //
 // On B200, 8192 x 50257: k = 8 0.278 ms (5.9 TB/s, 90 % of the copy rate), k = 64
 // 0.331 ms (5.0 TB/s), k = 256 0.62 ms, where lists outgrow one warp's registers;
+// 7615 x 1261, k = 24, a warp a row: 26 us;
 // 37 x 32003, k = 20, cut among clusters: 9.4 us. What passes costs issue slots
 // beside the loads. Tried: the row resident in a cluster's shared memory (0.66 ms,
 // its latencies are not hidden), a cp.async ring (0.57 ms), 128 threads (the same).
@@ -58,7 +59,7 @@ struct Smem {
 constexpr int SMALL = 512;
 
 template <int PER>
-__device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
+__device__ uint32_t select_part(u64 *buf, int n, int k) {
     const int lane = threadIdx.x & 31;
     uint32_t key[PER], top = 0, bottom = 0xFFFFFFFFu;
 #pragma unroll
@@ -113,11 +114,13 @@ __device__ void select_small(u64 *buf, int n, int k, Smem &sm) {
         at += __popc(mask);
         __syncwarp();
     }
-    if (lane == 0) {
-        sm.count = k;
-        // between NaN (0) and -inf lies no logit: k numbers, what follows has to exceed -inf
-        sm.low = lo == 0u ? 0u : max(lo, RANK_NEG_INF);
-    }
+    // between NaN (0) and -inf lies no logit: k numbers, what follows has to exceed -inf
+    return lo == 0u ? 0u : max(lo, RANK_NEG_INF);
+}
+
+// returns the new `low`
+__device__ __forceinline__ uint32_t select_small(u64 *buf, int n, int k) {
+    return n <= 128 ? select_part<4>(buf, n, k) : n <= 256 ? select_part<8>(buf, n, k) : select_part<SMALL / 32>(buf, n, k);
 }
 
 // Cuts the n > k candidates in buf to the k largest (any order) and sets low.
@@ -128,9 +131,11 @@ __device__ void select_k(u64 *buf, int n, int k, Smem &sm) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (n <= SMALL) {
         if (warp == 0) {
-            if (n <= 128) select_small<4>(buf, n, k, sm);
-            else if (n <= 256) select_small<8>(buf, n, k, sm);
-            else select_small<SMALL / 32>(buf, n, k, sm);
+            const uint32_t low = select_small(buf, n, k);
+            if (lane == 0) {
+                sm.count = k;
+                sm.low = low;
+            }
         }
         __syncthreads();
         return;
@@ -366,10 +371,105 @@ topk_kernel(const float *__restrict__ logits, long ldl, int V, int k, float *__r
     }
 }
 
+// Short rows: a warp each, ROWS of them a block. The bar is the k-th largest of 128
+// maxima, of every lane one for each place in its groups of four, so at least k
+// logits reach it; a second reading (from L1) collects those that do.
+constexpr int ROWS = 4;
+
+__global__ void __launch_bounds__(32 * ROWS)
+topk_warp_kernel(const float *__restrict__ logits, long ldl, int rows, int V, int k, float *__restrict__ values,
+                 int *__restrict__ indices) {
+    __shared__ u64 bufs[ROWS][SMALL];
+    const int lane = threadIdx.x & 31;
+    const long row = (long)blockIdx.x * ROWS + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    u64 *buf = bufs[threadIdx.x >> 5];
+    const float *x = logits + row * ldl;
+    const int head = min(V, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (V - head) / 4, tail = head + 4 * quads;
+    const float4 *x4 = (const float4 *)(x + head);
+    uint32_t key[4];
+    {
+        float4 m = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll 4
+        for (int q = lane; q < quads; q += 32) {
+            const float4 v = __ldg(x4 + q);
+            m.x = fmaxf(m.x, v.x);
+            m.y = fmaxf(m.y, v.y);
+            m.z = fmaxf(m.z, v.z);
+            m.w = fmaxf(m.w, v.w);
+        }
+        key[0] = rank_key(m.x);
+        key[1] = rank_key(m.y);
+        key[2] = rank_key(m.z);
+        key[3] = rank_key(m.w);
+    }
+    // the lowest rank that is taken, 0 with NaN
+    uint32_t least = 0, top = __reduce_max_sync(0xffffffffu, max(max(key[0], key[1]), max(key[2], key[3])));
+    while (least < top) {
+        const uint32_t mid = least + (top - least) / 2 + 1;
+        const int c = __reduce_add_sync(0xffffffffu, (key[0] >= mid) + (key[1] >= mid) + (key[2] >= mid) + (key[3] >= mid));
+        if (c >= k) least = mid;
+        else top = mid - 1;
+        if (c == k) break;
+    }
+    if (least <= RANK_NEG_INF) least = 0;  // too few numbers: NaN may count
+    int n = 0;
+    // takes one logit of every lane, of index i
+    auto take = [&](bool here, float e, int i) {
+        const uint32_t r = rank_key(e), mask = __ballot_sync(0xffffffffu, here && r >= least);
+        if (!mask) return;
+        if (here && r >= least) buf[n + __popc(mask & ((1u << lane) - 1))] = make_key(e, (uint32_t)i);
+        n += __popc(mask);
+    };
+    // leaves room for 128; later logits have to exceed the worst one kept
+    auto room = [&] {
+        __syncwarp();
+        if (n + 128 <= SMALL) return;
+        least = select_small(buf, n, k) + 1;
+        n = k;
+        __syncwarp();
+    };
+    take(lane < head, lane < head ? x[lane] : 0.0f, lane);
+    const float bar = least > RANK_NEG_INF ? rank_value(least) : 0.0f;
+    for (int q0 = 0; q0 < quads; q0 += 32) {
+        const int q = q0 + lane;
+        const bool here = q < quads;
+        const float4 v = here ? __ldg(x4 + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (least > RANK_NEG_INF && !__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bar)) continue;
+        const int i = head + 4 * q;
+        room();
+        take(here, v.x, i);
+        take(here, v.y, i + 1);
+        take(here, v.z, i + 2);
+        take(here, v.w, i + 3);
+    }
+    room();
+    take(tail + lane < V, tail + lane < V ? x[tail + lane] : 0.0f, tail + lane);
+    __syncwarp();
+    if (n > k) select_small(buf, n, k);
+    __syncwarp();
+    for (int c = lane; c < k; c += 32) {
+        const u64 mine = buf[c];
+        int r = 0;
+        for (int j = 0; j < k; ++j) r += buf[j] > mine;
+        values[row * k + r] = rank_value((uint32_t)(mine >> 32));
+        indices[row * k + r] = (int)(0xFFFFFFFFu - (uint32_t)mine);
+    }
+}
+
 }  // namespace
 
 int topk_rows(const float *logits, long ldl, int rows, int V, int k, float *values, int *indices, cudaStream_t s) {
     if (rows <= 0) return OK;
+    // Short rows leave a block's warps waiting for one another. A warp each takes
+    // 7000 x 500, k = 24 in 16 us where blocks take 80, 7000 x 2600 in 40, 51; but 600 x
+    // 2600 in 12.8, 7.8, and 7000 x 5000, k = 64 in 83, 78.
+    if (k <= 128 && (V <= 512 || (V <= 4096 && rows >= 12 * num_sms()))) {
+        topk_warp_kernel<<<(rows + ROWS - 1) / ROWS, 32 * ROWS, 0, s>>>(logits, ldl, rows, V, k, values, indices);
+        ++g_launch_count;
+        CG_CUDA(cudaGetLastError());
+        return OK;
+    }
     // Few rows leave SMs idle: cut each among up to 8 blocks, as long as a stretch
     // is a chunk or more and the stretches' k candidates fit one block's buffer.
     int parts = 1;

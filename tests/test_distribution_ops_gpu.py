@@ -314,6 +314,26 @@ def test_topk_many_rows(lib, cuda):
     check_topk(lib, logits(700, 3001, 11), 33)
 
 
+@pytest.mark.parametrize("rows,V,k", [(1783, 7, 7), (1783, 130, 128), (1783, 512, 100), (1779, 513, 128), (1783, 1300, 24),
+                                      (1778, 4096, 128), (1778, 4096, 1), (30, 400, 60), (1778, 4095, 129)])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_topk_many_short_rows(lib, cuda, rows, V, k, shift):
+    g = np.random.default_rng(V + k)
+    x = logits(rows, V, V)
+    x[0] = g.integers(-3, 3, V)
+    x[1] = 0.0
+    x[2] = np.arange(V)
+    x[3] = -np.arange(V)
+    x[4], x[5] = -INF, NAN
+    x[6, g.random(V) < 0.9], x[7, g.random(V) < 0.9] = -INF, NAN
+    x[8, V // 3:], x[9, : V // 2] = NAN, -INF
+    x[10, g.integers(0, V, 3)] = INF
+    x[11] = np.where(np.arange(V) % 2, 0.0, -0.0)
+    x[12, : V - 1] = NAN
+    x[rows - 1] = np.sort(x[rows - 1])
+    check_topk(lib, x, k, V + shift, shift)
+
+
 # ------------------------------------------------------------------ distill
 def ref_distill(x, tv, ti, tgt, tau, alpha, scale):
     """(loss, row_loss, dlogits, gradient's terms in size, largest |x - max|)."""
@@ -432,6 +452,19 @@ def test_distill_sizes(lib, cuda, V, k, rows, tau, alpha):
     assert a[0] == b[0] and np.array_equal(a[1], b[1])  # the loss is the same without its gradient
     c = check_distill(lib, x, tv, ti, tgt, tau, alpha, inplace=True)
     assert np.array_equal(a[2], c[2])
+
+
+@pytest.mark.parametrize("rows,V,k,ld,shift", [(1783, 5, 3, 5, 0), (1783, 513, 40, 515, 1), (1779, 1300, 8, 1300, 0),
+                                               (1778, 4096, 64, 4096, 2), (297, 4096, 1024, 4099, 0), (297, 4097, 16, 4097, 3)])
+def test_distill_many_short_rows(lib, cuda, rows, V, k, ld, shift):
+    tv, ti, tgt = teacher(rows, V, k, V)
+    x = logits(rows, V, k)
+    x[5], ti[6], tgt[7] = -INF, -1, -1
+    ti[8, : k // 2 + 1] = ti[8, 0]  # one token many times
+    a = check_distill(lib, x, tv, ti, tgt, 2.0, 0.5, ld=ld, shift=shift)
+    b = check_distill(lib, x, tv, ti, tgt, 2.0, 0.5, grad=False, ld=ld, shift=shift)
+    assert a[0] == b[0] and np.array_equal(a[1], b[1])
+    check_distill(lib, x, tv, ti, tgt, 1.0, 0.7, inplace=True, ld=ld, shift=shift)
 
 
 @pytest.mark.parametrize("ld,shift,ldd", [(1003, 0, 1003), (1003, 1, 1003), (1004, 2, 1007), (1010, 3, 1003)])
