@@ -20,7 +20,7 @@
 // four blocks an SM do not hide; the exponentials take half of the special-function
 // units' time. Two to seven more warps took 0.68 to 1.09 ms, shorter stretches 1.06,
 // sums of chunks while the next ones arrive 8 % more, clusters that prefetch their
-// next row three times as long.
+// next row three times as long. Short rows have a warp each: 7000 x 500 18 us.
 #include <algorithm>
 #include <cmath>
 
@@ -36,8 +36,8 @@ namespace coop = cooperative_groups;
 
 #define LAUNCH_CHECK() do { ++g_launch_count; CG_CUDA(cudaGetLastError()); } while (0)
 
-constexpr int COPY = 256;      // threads of the stretch, behind
-constexpr int NT = 32 + COPY;  // the list's warp
+constexpr int COPY = 256;  // threads of a stretch, behind the list's warp
+constexpr int ROWS = 4;    // of a block whose warps have a row each
 constexpr int MAX_PARTS = 8;
 constexpr int SLICE_BYTES = 52 * 1024;  // of a row in a block's shared memory: four blocks an SM
 constexpr float LOG2E = 1.4426950408889634f;
@@ -71,7 +71,7 @@ __device__ __forceinline__ void raise(Stats &s, float m, float ct) {
 struct DistillArgs {
     const float *logits;
     long ldl;
-    int V, stretch;
+    int rows, V, stretch;
     const float *tv;
     const int *ti;
     int k;
@@ -82,33 +82,48 @@ struct DistillArgs {
     long ldd;
 };
 
+// of shared memory: the stretch and the list
+__host__ __device__ __forceinline__ size_t row_bytes(int stretch, int k) {
+    return (((size_t)stretch + 8) * 4 + (size_t)k * 12 + 15) / 16 * 16;
+}
+
 // Cluster of 1 to 8 blocks per row, a stretch of it each. BOTH: the hard part's
 // softmax (temperature 1) is needed beside the list's. Warp 0 looks after the
 // list; until the first barrier the others read from shared memory only what they
 // copied there themselves.
-template <bool GRAD, bool BOTH>
-__global__ void __launch_bounds__(NT)
+// ALONE: one warp does all of it for a whole row, ROWS of them a block.
+template <bool GRAD, bool BOTH, bool ALONE>
+__global__ void __launch_bounds__(ALONE ? 32 * ROWS : 32 + COPY)
 distill_kernel(DistillArgs a) {
+    constexpr int NT = ALONE ? 32 : 32 + COPY, STEP = ALONE ? 32 : COPY;
     extern __shared__ float4 slice4[];  // [stretch + 8], then the list: sp, sx, si [k]
-    __shared__ Stats sw[NT / 32], sc[MAX_PARTS];
-    __shared__ int soft_list, twice, listed;
-    float *slice = (float *)slice4, *sp = slice + a.stretch + 8, *sx = sp + a.k;
+    __shared__ Stats sw_of[ALONE ? ROWS : NT / 32], sc[MAX_PARTS];
+    __shared__ int flags[ALONE ? ROWS : 1][3];
+    const int own = ALONE ? threadIdx.x >> 5 : 0;  // of the block's rows
+    Stats *sw = sw_of + own;
+    int &soft_list = flags[own][0], &twice = flags[own][1], &listed = flags[own][2];
+    float *slice = (float *)((char *)slice4 + own * row_bytes(a.stretch, a.k)), *sp = slice + a.stretch + 8, *sx = sp + a.k;
     int *si = (int *)(sx + a.k);
     auto cluster = coop::this_cluster();
     const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
     if (parts > 1) cluster.barrier_arrive();  // waited for before the first write to another block
-    const long row = blockIdx.x / parts;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long row = ALONE ? (long)blockIdx.x * ROWS + own : blockIdx.x / parts;
+    if (ALONE && row >= a.rows) return;
+    auto sync = [] {
+        if (ALONE) __syncwarp();
+        else __syncthreads();
+    };
+    const int tid = ALONE ? threadIdx.x & 31 : threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int lo = min(a.V, part * a.stretch), hi = min(a.V, lo + a.stretch), n = hi - lo, k = a.k;
     const float *xr = a.logits + row * a.ldl, *x = xr + lo;
     const float ct = LOG2E / a.tau;
     // elements before the first 16-byte boundary, whole groups of four, the rest;
     // element i of the stretch is kept at slice[pad + i], groups at float4s
     const int head = min(n, (int)(((16 - (uintptr_t)x % 16) / 4) % 4)), quads = (n - head) / 4, pad = (4 - head) & 3;
-    const int at = tid - 32;  // among the threads of the stretch
+    const int at = ALONE ? tid : tid - 32;  // among the threads of the stretch
     const int odd = at < 0 ? -1 : at < head ? at : at < n - 4 * quads ? at + 4 * quads : -1;  // this thread's of those at both ends
     float4 *s4 = (float4 *)(slice + pad + head);
-    for (int q = at; at >= 0 && q < quads; q += COPY)
+    for (int q = at; at >= 0 && q < quads; q += STEP)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s4 + q)), "l"(x + head + 4 * q) : "memory");
     if (odd >= 0)
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slice + pad + odd)), "l"(x + odd) : "memory");
@@ -135,7 +150,7 @@ distill_kernel(DistillArgs a) {
 
     // statistics of the thread, the warp, the block and the row, in a fixed order
     Stats s{-INFINITY, 0.0f, 0.0f};
-    for (int q = at; at >= 0 && q < quads; q += COPY) {
+    for (int q = at; at >= 0 && q < quads; q += STEP) {
         const float4 v = s4[q];
         s.m = fmaxf(s.m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
@@ -147,7 +162,7 @@ distill_kernel(DistillArgs a) {
             if (BOTH) s.s1 += ex2(fmaf(v, LOG2E, -r1));
         };
 #pragma unroll 2
-        for (int q = at; at >= 0 && q < quads; q += COPY) {
+        for (int q = at; at >= 0 && q < quads; q += STEP) {
             const float4 v = s4[q];
             add(v.x);
             add(v.y);
@@ -161,7 +176,7 @@ distill_kernel(DistillArgs a) {
     }
     if (lane == 0) sw[warp] = s;
     if (tid == 0) soft_list = lm > -INFINITY;
-    __syncthreads();
+    sync();
     auto join = [&](const Stats *v, int count) {
         float m = v[0].m;
         for (int w = 1; w < count; ++w) m = fmaxf(m, v[w].m);
@@ -216,17 +231,17 @@ distill_kernel(DistillArgs a) {
         return none ? 0.0f : g;
     };
     if (odd >= 0) d[odd] = grad(slice[pad + odd]);
-    if (((uintptr_t)(d + head) & 15) == 0 && warp > 0) {  // the groups of x are groups of d too
+    if (((uintptr_t)(d + head) & 15) == 0 && at >= 0) {  // the groups of x are groups of d too
 #pragma unroll 2
-        for (int q = at; q < quads; q += COPY) {
+        for (int q = at; q < quads; q += STEP) {
             const float4 v = s4[q];
             __stcs((float4 *)(d + head) + q, make_float4(grad(v.x), grad(v.y), grad(v.z), grad(v.w)));
         }
-    } else if (warp > 0) {  // another alignment: element by element, from the whole block's copies
-        for (int i = head + at; i < head + 4 * quads; i += COPY) d[i] = grad(slice[pad + i]);
+    } else if (at >= 0) {  // another alignment: element by element, from the whole block's copies
+        for (int i = head + at; i < head + 4 * quads; i += STEP) d[i] = grad(slice[pad + i]);
     }
     if (none) return;
-    __syncthreads();
+    sync();
     // entries of the list and the target in this stretch: written again with
     // their own part taken off, by the first entry of a token for all of its
     if (warp != 0) return;
@@ -286,18 +301,19 @@ loss_sum_kernel(const float *__restrict__ row_loss, int rows, float scale, float
     if (threadIdx.x == 0) *loss = scale * sh[0];
 }
 
-template <bool GRAD, bool BOTH>
-int launch(const DistillArgs &a, int rows, int parts, size_t smem, cudaStream_t s) {
+template <bool GRAD, bool BOTH, bool ALONE>
+int launch_as(const DistillArgs &a, int rows, int parts, cudaStream_t s) {
     static bool set = false;
     if (!set) {
-        CG_CUDA(cudaFuncSetAttribute(distill_kernel<GRAD, BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     ROW_MAX_VOCAB / MAX_PARTS * 4 + 64 + 12 * TOPK_MAX));
+        CG_CUDA(cudaFuncSetAttribute(distill_kernel<GRAD, BOTH, ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     ALONE ? ROWS * (4096 * 4 + 64 + 12 * TOPK_MAX)
+                                           : ROW_MAX_VOCAB / MAX_PARTS * 4 + 64 + 12 * TOPK_MAX));
         set = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * parts));
-    cfg.blockDim = dim3(NT);
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(ALONE ? (unsigned)((rows + ROWS - 1) / ROWS) : (unsigned)(rows * parts));
+    cfg.blockDim = dim3(ALONE ? 32 * ROWS : 32 + COPY);
+    cfg.dynamicSmemBytes = row_bytes(a.stretch, a.k) * (ALONE ? ROWS : 1);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -305,9 +321,14 @@ int launch(const DistillArgs &a, int rows, int parts, size_t smem, cudaStream_t 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    CG_CUDA(cudaLaunchKernelEx(&cfg, distill_kernel<GRAD, BOTH>, a));
+    CG_CUDA(cudaLaunchKernelEx(&cfg, distill_kernel<GRAD, BOTH, ALONE>, a));
     ++g_launch_count;
     return OK;
+}
+
+template <bool GRAD, bool BOTH>
+int launch(const DistillArgs &a, int rows, int parts, bool alone, cudaStream_t s) {
+    return alone ? launch_as<GRAD, BOTH, true>(a, rows, parts, s) : launch_as<GRAD, BOTH, false>(a, rows, parts, s);
 }
 
 }  // namespace
@@ -323,16 +344,19 @@ int distill_rows(const float *logits, long ldl, int rows, int V, const float *tv
     while (parts < MAX_PARTS && ((long)V * 4 > (long)parts * SLICE_BYTES ||
                                  ((long)rows * parts * 2 <= num_sms() && V >= parts * 4096)))
         parts *= 2;
+    // Short rows of which every SM gets some leave a block's warps waiting for one
+    // another: a warp each (7000 x 500 with gradient 18 us, 61 by blocks; 7000 x 2600 47
+    // us, 80; 600 x 2600 11.8 us, 13.8; 150 x 2600 10.4, 8.5).
+    const bool alone = parts == 1 && (V <= 512 || (V <= 4096 && rows >= 2 * num_sms()));
     if ((long)rows * parts > 0x7FFFFFFFL) {
         set_last_error(ERR_ARG, "distill: %d rows are too many", rows);
         return ERR_ARG;
     }
-    DistillArgs a{logits, ldl, V, ((V + parts - 1) / parts + 3) / 4 * 4, tv, ti, k, targets, tau, alpha, scale, row_loss,
+    DistillArgs a{logits, ldl, rows, V, ((V + parts - 1) / parts + 3) / 4 * 4, tv, ti, k, targets, tau, alpha, scale, row_loss,
                   dlogits, ldd};
-    const size_t smem = ((size_t)a.stretch + 8) * sizeof(float) + (size_t)k * 12;
     if (alpha < 1.0f && targets)
-        return dlogits ? launch<true, true>(a, rows, parts, smem, s) : launch<false, true>(a, rows, parts, smem, s);
-    return dlogits ? launch<true, false>(a, rows, parts, smem, s) : launch<false, false>(a, rows, parts, smem, s);
+        return dlogits ? launch<true, true>(a, rows, parts, alone, s) : launch<false, true>(a, rows, parts, alone, s);
+    return dlogits ? launch<true, false>(a, rows, parts, alone, s) : launch<false, false>(a, rows, parts, alone, s);
 }
 
 int distill_loss_sum(const float *row_loss, int rows, float scale, float *loss, cudaStream_t s) {
