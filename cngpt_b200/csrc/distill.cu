@@ -303,15 +303,17 @@ loss_sum_kernel(const float *__restrict__ row_loss, int rows, float scale, float
 
 template <bool GRAD, bool BOTH, bool ALONE>
 int launch_as(const DistillArgs &a, int rows, int parts, cudaStream_t s) {
-    static bool set = false;
-    if (!set) {
+    static bool set_on[MAX_DEVICES];
+    bool *set;
+    CG_TRY(this_device(set_on, &set));
+    if (!*set) {
         CG_CUDA(cudaFuncSetAttribute(distill_kernel<GRAD, BOTH, ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      ALONE ? ROWS * (4096 * 4 + 64 + 12 * TOPK_MAX)
                                            : ROW_MAX_VOCAB / MAX_PARTS * 4 + 64 + 12 * TOPK_MAX));
-        set = true;
+        *set = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ALONE ? (unsigned)((rows + ROWS - 1) / ROWS) : (unsigned)(rows * parts));
+    cfg.gridDim = dim3(ALONE ? (unsigned)((rows - 1) / ROWS + 1) : (unsigned)(rows * parts));
     cfg.blockDim = dim3(ALONE ? 32 * ROWS : 32 + COPY);
     cfg.dynamicSmemBytes = row_bytes(a.stretch, a.k) * (ALONE ? ROWS : 1);
     cfg.stream = s;

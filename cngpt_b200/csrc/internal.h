@@ -174,4 +174,8 @@ extern unsigned long long g_launch_count;
 
 int num_sms();
 
+// A kernel's attributes belong to a device: *flag is the current one's entry of `of`.
+constexpr int MAX_DEVICES = 64;
+int this_device(bool (&of)[MAX_DEVICES], bool **flag);
+
 }  // namespace cg

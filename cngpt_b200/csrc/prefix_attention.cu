@@ -629,11 +629,13 @@ int launch_prefix(const PrefixAttn &a, const Parts &w, cudaStream_t s) {
     using Cfg = PrefixCfg<HSP, RG>;
     constexpr size_t smem = (size_t)Cfg::FLOATS * sizeof(float);
     static_assert(smem <= 227 * 1024, "shared memory of a block");
-    static bool set = false;
-    if (!set) {
+    static bool set_on[MAX_DEVICES];
+    bool *set;
+    CG_TRY(this_device(set_on, &set));
+    if (!*set) {
         CG_CUDA(cudaFuncSetAttribute(prefix_part_kernel<HSP, RG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)smem));
-        set = true;
+        *set = true;
     }
     const long R = (long)a.B * (a.H / a.Hk), n_tiles = (R + 16 * RG - 1) / (16 * RG);
     const bool vec = a.hs % 4 == 0 && a.ldp % 4 == 0 && ((uintptr_t)a.pk | (uintptr_t)a.pv) % 16 == 0;

@@ -76,4 +76,15 @@ int num_sms() {
     return g_sms;
 }
 
+int this_device(bool (&of)[MAX_DEVICES], bool **flag) {
+    int dev = 0;
+    CG_CUDA(cudaGetDevice(&dev));
+    if (dev >= MAX_DEVICES) {
+        set_last_error(ERR_ARG, "device %d: more than %d are not supported", dev, MAX_DEVICES);
+        return ERR_ARG;
+    }
+    *flag = &of[dev];
+    return OK;
+}
+
 }  // namespace cg

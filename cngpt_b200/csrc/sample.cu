@@ -926,11 +926,13 @@ int sample_rows(const SampleRows &a, cudaStream_t s) {
     const int stretch = ((a.V + parts - 1) / parts + 3) / 4 * 4;
     int sh = 50;
     while ((a.V - 1) >> (62 - sh)) --sh;  // V weights of 2^sh stay below 2^62
-    static bool set = false;
-    if (!set) {
+    static bool set_on[MAX_DEVICES];
+    bool *set;
+    CG_TRY(this_device(set_on, &set));
+    if (!*set) {
         CG_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (SAMPLE_MAX_VOCAB / MAX_PARTS + 16) * 4));
-        set = true;
+        *set = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * parts));

@@ -465,7 +465,7 @@ int topk_rows(const float *logits, long ldl, int rows, int V, int k, float *valu
     // 7000 x 500, k = 24 in 16 us where blocks take 80, 7000 x 2600 in 40, 51; but 600 x
     // 2600 in 12.8, 7.8, and 7000 x 5000, k = 64 in 83, 78.
     if (k <= 128 && (V <= 512 || (V <= 4096 && rows >= 12 * num_sms()))) {
-        topk_warp_kernel<<<(rows + ROWS - 1) / ROWS, 32 * ROWS, 0, s>>>(logits, ldl, rows, V, k, values, indices);
+        topk_warp_kernel<<<(rows - 1) / ROWS + 1, 32 * ROWS, 0, s>>>(logits, ldl, rows, V, k, values, indices);
         ++g_launch_count;
         CG_CUDA(cudaGetLastError());
         return OK;
@@ -480,11 +480,13 @@ int topk_rows(const float *logits, long ldl, int rows, int V, int k, float *valu
         return ERR_ARG;
     }
     const size_t smem = (size_t)(std::max(2 * k, TRIGGER) + CHUNK + 8) * sizeof(u64);
-    static bool set = false;
-    if (!set) {
+    static bool set_on[MAX_DEVICES];
+    bool *set;
+    CG_TRY(this_device(set_on, &set));
+    if (!*set) {
         CG_CUDA(cudaFuncSetAttribute(topk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)((2 * TOPK_MAX + CHUNK + 8) * sizeof(u64))));
-        set = true;
+        *set = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * parts));
