@@ -14,15 +14,16 @@
 //                       sequence only, so its bytes set the time;
 //   join_kernel         a query's triples, in the order of the stretches.
 //
-// The three are chained by programmatic dependent launch, so the suffix blocks
+//
+// Few keys take direct_kernel alone. The three are chained by programmatic dependent launch, so the suffix blocks
 // fill the SMs that the prefix blocks leave.
 //
 // On B200: 48 samples x 16 heads of 64 over 16384 shared keys and up to 512 own (36 us
 // of bytes): 94 us, of which the prefix takes 76 us at half the tf32 mma.sync rate
 // (276 TFLOP/s measured; three products a product), the suffixes partly beside it;
 // 16 samples x 12 heads, 768 + 255 keys (4.6 us of bytes): 13.1 us; 12 samples x 24
-// heads of 128 over 6, 5003 + 77 keys (5.2 us): 31 us; one sample, 109 keys: 6.4 us,
-// three launches. fp16 products with scaled rows need half the tensor time and gave
+// heads of 128 over 6, 5003 + 77 keys (5.2 us): 31 us; one sample, 109 keys: 4.0 us
+// in one launch (direct_kernel). fp16 products with scaled rows need half the tensor time and gave
 // half the error, but took as long: splitting the rows then sets the pace.
 #include <algorithm>
 #include <cmath>
@@ -503,6 +504,109 @@ suffix_part_kernel(PrefixAttn a, Parts w, bool vec) {
     pdl_wait();  // the prefix blocks: the kernel that waits for this one waits for them too
 }
 
+// ------------------------------------------------------------------ direct
+// Few keys: one block does a query's all of them, prefix and suffix, in one launch
+// without the workspace; the prefix comes from L2 as often as there are queries.
+// The lanes of one key's row keep their own (m, l, o), joined at the end in the order
+// of lanes and warps.
+constexpr int DWARPS = 16;
+
+template <int LPK, int NF>
+__global__ void __launch_bounds__(DWARPS * 32, 1)
+direct_kernel(PrefixAttn a, bool vec) {
+    constexpr int KPI = 32 / LPK, ITER = 8 / NF;
+    __shared__ float so[DWARPS][LPK * 4 * NF];
+    __shared__ float2 sml[DWARPS];
+    const int h = blockIdx.x % a.H, b = blockIdx.x / a.H, hs = a.hs;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPK, li = lane % LPK;
+    const int n = a.P + (a.S > 0 ? min(max(a.suffix_len[b], 0), a.S) : 0);
+    const long head = (long)(h / (a.H / a.Hk)) * hs, own = b * a.seq_stride;
+    const float sc = a.scale * LOG2E, *qr = a.q + b * a.ldq + (long)h * hs;
+    float4 q[NF], o[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        q[f] = row4(qr, (li + f * LPK) * 4, hs, true, false);
+        o[f] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int t = warp * KPI * ITER; t < n; t += DWARPS * KPI * ITER) {
+        float4 k[ITER][NF], v[ITER][NF];
+        float s[ITER] = {};
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const int j = t + i * KPI + sub;
+            const long at = head + (j < a.P ? (long)j * a.ldp : own + (long)(j - a.P) * a.lds);
+            const float *kr = (j < a.P ? a.pk : a.sk) + at, *vr = (j < a.P ? a.pv : a.sv) + at;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                k[i][f] = row4(kr, (li + f * LPK) * 4, hs, j < n, vec);
+                v[i][f] = row4(vr, (li + f * LPK) * 4, hs, j < n, vec);
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+                s[i] = fmaf(q[f].x, k[i][f].x, fmaf(q[f].y, k[i][f].y, fmaf(q[f].z, k[i][f].z, fmaf(q[f].w, k[i][f].w, s[i]))));
+#pragma unroll
+            for (int x = LPK / 2; x > 0; x >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], x);
+            s[i] = t + i * KPI + sub < n ? s[i] * sc : -INFINITY;
+            mx = fmaxf(mx, s[i]);
+        }
+        const float ref = mx == -INFINITY ? 0.0f : mx, c = ex2(m - ref);
+        m = mx;
+        l *= c;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) o[f] = make_float4(o[f].x * c, o[f].y * c, o[f].z * c, o[f].w * c);
+#pragma unroll
+        for (int i = 0; i < ITER; ++i) {
+            const float p = ex2(s[i] - ref);
+            l += p;
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+                o[f] = make_float4(fmaf(p, v[i][f].x, o[f].x), fmaf(p, v[i][f].y, o[f].y), fmaf(p, v[i][f].z, o[f].z),
+                                   fmaf(p, v[i][f].w, o[f].w));
+        }
+    }
+    // the warp's, then the block's
+    float wm = m;
+#pragma unroll
+    for (int x = LPK; x < 32; x <<= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, x));
+    const float c = ex2(m - (wm == -INFINITY ? 0.0f : wm));
+    l *= c;
+#pragma unroll
+    for (int f = 0; f < NF; ++f) o[f] = make_float4(o[f].x * c, o[f].y * c, o[f].z * c, o[f].w * c);
+#pragma unroll
+    for (int x = LPK; x < 32; x <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            o[f].x += __shfl_xor_sync(0xffffffffu, o[f].x, x);
+            o[f].y += __shfl_xor_sync(0xffffffffu, o[f].y, x);
+            o[f].z += __shfl_xor_sync(0xffffffffu, o[f].z, x);
+            o[f].w += __shfl_xor_sync(0xffffffffu, o[f].w, x);
+        }
+    }
+    if (lane == 0) sml[warp] = make_float2(wm, l);
+    if (sub == 0)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) *(float4 *)&so[warp][(li + f * LPK) * 4] = o[f];
+    __syncthreads();
+    if ((int)threadIdx.x >= hs) return;
+    float mm = -INFINITY, ll = 0.0f, oo = 0.0f;
+#pragma unroll
+    for (int x = 0; x < DWARPS; ++x) mm = fmaxf(mm, sml[x].x);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+    for (int x = 0; x < DWARPS; ++x) {
+        const float f = ex2(sml[x].x - ref);
+        ll = fmaf(sml[x].y, f, ll);
+        oo = fmaf(so[x][threadIdx.x], f, oo);
+    }
+    a.out[b * a.ldo + (long)h * hs + threadIdx.x] = n > 0 ? oo / ll : 0.0f;
+}
+
 // -------------------------------------------------------------------- join
 constexpr int JT = 128, JBATCH = 4;
 
@@ -679,6 +783,19 @@ size_t prefix_attention_ws_bytes(int B, int H, int Hk, int hs, int P, int S) {
 
 int prefix_attention(const PrefixAttn &a, void *ws, cudaStream_t s) {
     if (a.B <= 0) return OK;
+    // One launch where that is no longer than three: 109 keys, 12 queries 4.0 us (6.6),
+    // 16 x 12 queries 6.9 (8.2), 355 keys 11.0 (11.1); but 528 keys 14.7 (10.7), and
+    // 48 x 12 queries, four rounds of blocks, 109 keys 12.7 (12.1).
+    if ((long)a.P + a.S <= 384 && (long)a.B * a.H <= 2 * num_sms()) {
+        const bool vec = a.hs % 4 == 0 &&
+                         (a.P == 0 || (a.ldp % 4 == 0 && ((uintptr_t)a.pk | (uintptr_t)a.pv) % 16 == 0)) &&
+                         (a.S == 0 || ((a.lds | a.seq_stride) % 4 == 0 && ((uintptr_t)a.sk | (uintptr_t)a.sv) % 16 == 0));
+        auto go = [&](auto kernel) { return launch_pdl(kernel, (long)a.B * a.H, DWARPS * 32, 0, false, s, a, vec); };
+        if (a.hs <= 32) return go(direct_kernel<8, 1>);
+        if (a.hs <= 64) return go(direct_kernel<16, 1>);
+        if (a.hs <= 128) return go(direct_kernel<32, 1>);
+        return go(direct_kernel<32, 2>);
+    }
     Parts w = plan(a.B, a.H, a.Hk, a.hs, a.P, a.S);
     w.o = (float *)ws;
     const size_t rows = (size_t)(w.n_pre + w.n_suf) * a.B * a.H;

@@ -114,6 +114,26 @@ def test_head_layouts(lib, cuda, H, Hk, hs):
         Case(B, H, Hk, hs, P, S, seed=hs).check(lib)
 
 
+@pytest.mark.parametrize("H,Hk,hs", [(1, 1, 1), (3, 3, 8), (2, 1, 7), (4, 2, 16), (6, 6, 20), (8, 2, 32), (5, 5, 33), (25, 25, 64),
+                                     (12, 1, 64), (6, 2, 80), (24, 6, 128), (3, 1, 131), (4, 2, 256)])
+def test_head_layouts_beyond_one_block(lib, cuda, H, Hk, hs):
+    for B, P, S in ((1, 385, 3), (5, 449, 40), (17, 321, 70)):
+        Case(B, H, Hk, hs, P, S, lens=[(7 * i) % (S + 1) for i in range(B)], seed=H).check(lib)
+
+
+@pytest.mark.parametrize("P,S", [(1, 0), (0, 1), (1, 1), (63, 1), (64, 64), (65, 5), (127, 130), (384, 0), (383, 1), (384, 1),
+                                 (0, 385)])
+@pytest.mark.parametrize("B", [2, 25])
+def test_lengths_on_both_sides_of_one_block(lib, cuda, P, S, B):
+    Case(B, 12, 12, 64, P, S, lens=np.arange(B) % (S + 1), seed=P + S).check(lib)
+
+
+@pytest.mark.parametrize("pad", [1, 2, 4])
+def test_pitches_beyond_one_block(lib, cuda, pad):
+    Case(6, 4, 4, 64, 400, 50, lens=[0, 50, 3, 17, 49, 1], pad=pad).check(lib)
+    Case(3, 4, 2, 20, 377, 50, lens=[0, 50, 3], pad=pad).check(lib)
+
+
 @pytest.mark.parametrize("B", [2, 7, 8, 9, 15, 17, 31, 32, 33, 63, 64, 65, 100, 129, 200])
 def test_batches(lib, cuda, B):
     Case(B, 2, 2, 64, 515, 20, seed=B).check(lib)
